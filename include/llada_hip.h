@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define LLADA_ABI_VERSION 4
+#define LLADA_ABI_VERSION 5
 
 #define LLADA_OK 0
 #define LLADA_ERR_INVALID (-1)      /* bad argument (the Python host raises AssertionError/ValueError) */
@@ -231,6 +231,45 @@ int llada_forward_block(const llada_config* cfg, const llada_weights* w, const i
                         size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Key/value cache in 8 bits and the attention that reads it.  No counterpart in the reference (see the block-cached
+ * forward above, whose cache it stands in for at a third of the memory).  One layer's cache is
+ * llada_kv8_layer_bytes(n_seq, seq_len, n_heads) bytes of caller memory, 256-byte aligned, holding the keys and
+ * values of n_seq sequences of seq_len tokens: codes of 8 bits in blocks of 64 consecutive tokens and one head, each
+ * block of keys and of values with one scale 2^k, k the smallest integer (>= -126) for which the block's largest
+ * magnitude is at most 448 * 2^k (LLADA_KV_E4M3: OCP float8 e4m3) or 127 * 2^k (LLADA_KV_INT8); k = 0 for an
+ * all-zero block.  code = x * 2^-k rounded to nearest even; the stored value code * 2^k is exact in bf16 (blocks whose
+ * values are below 2^-117 excepted).  Infinities saturate and do not enter the scale; a NaN stays one in e4m3 and
+ * becomes 0 in int8.  The order of the bytes inside is the library's own; llada_kv8_read gives the values.
+ * ------------------------------------------------------------------------------------------- */
+#define LLADA_KV_E4M3 0
+#define LLADA_KV_INT8 1
+size_t llada_kv8_layer_bytes(int32_t n_seq, int32_t seq_len, int32_t n_heads);
+
+/* Writes the tokens start .. start + len - 1 of every sequence: qkv holds n_seq * len bf16 rows [Q | K | V]
+ * (3 * n_heads * 128 columns, row stride row_stride elements, rows 16-byte aligned), of which K and V are read.
+ * key_mask [n_seq, seq_len] (1 = attend) or NULL: a masked token of a written block is stored as zeros and does not
+ * enter its scale.  A block that the range covers only in part is written anew from its new tokens and, for the others,
+ * from what the cache holds of them, so the first call on fresh memory covers 0 .. seq_len. */
+int llada_kv8_write(const void* qkv, int64_t row_stride, const uint8_t* key_mask, void* cache, int32_t kv_type, int32_t n_seq,
+                    int32_t seq_len, int32_t n_heads, int32_t start, int32_t len, void* stream);
+
+/* The values the cache stands for: k_out, v_out [n_seq * seq_len, n_heads * 128] bf16. */
+int llada_kv8_read(const void* cache, int32_t kv_type, void* k_out, void* v_out, int32_t n_seq, int32_t seq_len,
+                   int32_t n_heads, void* stream);
+
+/* llada_attn_bidir_queries_bf16 over such a cache: q [n_seq * n_q, q_stride] (head h at columns h * 128) over all seq_len
+ * tokens of the sequence, softmax(q k^T / sqrt(128)) v, out [n_seq * n_q, n_heads * 128] bf16.  block_qkv (may be NULL):
+ * bf16 [Q | K | V] rows [n_seq * block_len], row stride block_stride, whose keys and values stand in for the cached ones of
+ * the tokens block_start .. block_start + block_len - 1 (the cache is only read).  key_mask as above; what stands under a
+ * masked token, NaN included, does not reach the result, and a sequence without an unmasked token gives zeros.
+ * workspace (may be NULL; llada_attn_kv8_workspace_bytes; 16-byte aligned): scratch of this call with which the keys are
+ * dealt over several workgroups where the queries alone would leave most CUs idle. */
+int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, const void* cache, int32_t kv_type, const uint8_t* key_mask,
+                   void* out, int32_t n_seq, int32_t seq_len, int32_t n_heads, const void* block_qkv, int64_t block_stride,
+                   int32_t block_start, int32_t block_len, void* workspace, size_t workspace_bytes, void* stream);
+size_t llada_attn_kv8_workspace_bytes(int32_t n_seq, int32_t n_q, int32_t seq_len, int32_t n_heads);
+
+/* ---------------------------------------------------------------------------------------------
  * Sampler epilogue: replaces generate.py:81-134 after the forward.
  * ------------------------------------------------------------------------------------------- */
 
@@ -298,6 +337,39 @@ int llada_remask_scores(const llada_remask_args* args, void* stream);
  * entry a call reads was written by that call). */
 #define LLADA_STATIC_REMASK_MAX_ROWS 8192
 int llada_remask_scores_static(const llada_remask_args* args, void* stream);
+
+/* Truncated sampling.  No counterpart in the reference's sampler, whose temperature (generate.py:8-19) draws from the
+ * whole vocabulary.  With a row's entries ordered by (logit descending, index ascending), m the largest logit and
+ * w_i = exp((l_i - m) / temperature) in float64:
+ *   n_k = top_k (the whole row when 0), n_p = the smallest n with w_1 + .. + w_n >= top_p * (w_1 + .. + w_{n_k}),
+ *   n_m = the number of w_i >= min_p (taken as l_i - m >= temperature * log(min_p)), n = max(1, min(n_k, n_p, n_m)),
+ * the token is the first i with w_1 + .. + w_i > u * (w_1 + .. + w_n), u the row's uniform in [0, 1).  temperature 0: the
+ * arg-max.  Entries of -inf (and NaN) are never drawn; a row of nothing else gives token 0 with probability 0.
+ * The scalars are checked (temperature in [0, 1e30], top_k >= 0, top_p in (0, 1], min_p in [0, 1]); where an array is given
+ * (device memory, one value a row) it replaces the scalar, values outside those ranges acting like the nearest end. */
+typedef struct llada_sampling {
+    double temperature, top_p, min_p;
+    int32_t top_k;                  /* 0 = off */
+    const float* row_temperature;   /* [rows] or NULL */
+    const int32_t* row_top_k;
+    const float* row_top_p;
+    const float* row_min_p;
+    const double* uniforms;         /* float64 in [0, 1), or NULL = the library's Philox stream */
+} llada_sampling;
+
+/* tokens[r] (int64) and, unless NULL, probs[r] (float32: the token's probability among the kept entries) for each row
+ * of logits [n_rows, vocab] bf16, rows row_stride elements apart (uncond_logits likewise, or NULL: combined with
+ * cfg_scale as llada_remask_scores does).  Parameter arrays and uniforms: [n_rows].  vocab <= 131072 (131065 where rows
+ * are not 16-byte aligned).  Philox counters: (0, 0, row_offset + r, step). */
+int llada_sample_rows(const void* logits, const void* uncond_logits, int64_t row_stride, double cfg_scale, int32_t n_rows,
+                      int32_t vocab, const llada_sampling* sampling, uint64_t seed, uint32_t step, uint32_t row_offset,
+                      int64_t* tokens, float* probs, void* stream);
+
+/* llada_remask_scores with the candidate tokens drawn this way instead of by Gumbel-max (args->temperature, noise and the
+ * workspace are ignored): confidence is still the remasking rule on the row's whole temperature-1 softmax.
+ * uniforms: [B, L], by position; parameter arrays: [B].  Philox counters: (0, column, row_offset + b, step).
+ * logits 16-byte aligned, vocab a multiple of 8 up to 131072. */
+int llada_remask_scores_sampled(const llada_remask_args* args, const llada_sampling* sampling, void* stream);
 
 /* generate.py:130-134: per row b, the k = sched[b*sched_stride + step] largest confidences
  * (NaN ranks highest, ties go to the lower index) are transferred: x[b, i] = x0[b, i]. */

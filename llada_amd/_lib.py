@@ -11,7 +11,7 @@ import subprocess
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("LLADA_HIP_LIB") or os.path.join(_HERE, "libllada_hip.so")   # override: A/B timing of two builds
 
-ABI_VERSION = 4     # LLADA_ABI_VERSION of include/llada_hip.h this binding was written for
+ABI_VERSION = 5     # LLADA_ABI_VERSION of include/llada_hip.h this binding was written for
 OK = 0
 ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP, ERR_WORKSPACE = -1, -2, -3, -4
 
@@ -20,6 +20,7 @@ FLAG_LOGITS_EOS_INF, FLAG_CONF_EOS_EOT_INF, FLAG_CONF_FLOAT32 = 1, 2, 4
 EPI_PLAIN, EPI_RESIDUAL, EPI_ROPE_QKV, EPI_SWIGLU = 0, 1, 2, 3
 GEMM_W_TILED = 0x100
 STATIC_REMASK_MAX_ROWS = 8192
+KV_TYPES = {"e4m3": 0, "int8": 1}
 
 vp = C.c_void_p
 
@@ -42,6 +43,11 @@ class RemaskArgs(C.Structure):
                 ("eos_id", C.c_int32), ("eot_id", C.c_int32), ("temperature", C.c_float), ("noise", vp),
                 ("rand_scores", vp), ("seed", C.c_uint64), ("step", C.c_uint32), ("row_offset", C.c_uint32),
                 ("x0", vp), ("confidence", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", C.c_int32),
+                ("row_temperature", vp), ("row_top_k", vp), ("row_top_p", vp), ("row_min_p", vp), ("uniforms", vp)]
 
 
 # name -> (restype, argtypes); every symbol include/llada_hip.h declares
@@ -73,6 +79,12 @@ SIGNATURES = {
     "llada_forward_block_workspace_bytes": (C.c_size_t, [C.POINTER(Config), C.c_int32, C.c_int32, C.c_int32]),
     "llada_forward_block": (C.c_int, [C.POINTER(Config), C.POINTER(Weights), vp, vp, vp, vp, C.c_int32, C.c_int32,
                                       C.c_int32, C.c_int32, vp, C.c_int32, vp, C.c_int32, vp, vp, C.c_size_t, vp]),
+    "llada_kv8_layer_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
+    "llada_kv8_write": (C.c_int, [vp, C.c_int64, vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, vp]),
+    "llada_kv8_read": (C.c_int, [vp, C.c_int32, vp, vp, C.c_int32, C.c_int32, C.c_int32, vp]),
+    "llada_attn_kv8": (C.c_int, [vp, C.c_int64, C.c_int32, vp, C.c_int32, vp, vp, C.c_int32, C.c_int32, C.c_int32, vp, C.c_int64,
+                                 C.c_int32, C.c_int32, vp, C.c_size_t, vp]),
+    "llada_attn_kv8_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "llada_num_transfer_tokens": (C.c_int, [vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int32,
                                             vp, vp]),
     "llada_add_gumbel_noise": (C.c_int, [vp, vp, C.c_double, vp, C.c_int64, C.c_int32, C.c_int32, C.c_uint64, C.c_uint32,
@@ -80,6 +92,9 @@ SIGNATURES = {
     "llada_rows_workspace_bytes": (C.c_size_t, [C.c_int32]),
     "llada_remask_scores": (C.c_int, [C.POINTER(RemaskArgs), vp]),
     "llada_remask_scores_static": (C.c_int, [C.POINTER(RemaskArgs), vp]),
+    "llada_sample_rows": (C.c_int, [vp, vp, C.c_int64, C.c_double, C.c_int32, C.c_int32, C.POINTER(Sampling), C.c_uint64,
+                                    C.c_uint32, C.c_uint32, vp, vp, vp]),
+    "llada_remask_scores_sampled": (C.c_int, [C.POINTER(RemaskArgs), C.POINTER(Sampling), vp]),
     "llada_topk_transfer": (C.c_int, [vp, vp, vp, C.c_int32, C.c_int32, vp, C.c_int32, C.c_int32, vp]),
     "llada_ll_mask": (C.c_int, [vp, vp, C.c_int32, C.c_int32, C.c_int32, C.c_int64, vp, vp, C.c_uint64, C.c_uint32,
                                 C.c_uint32, vp]),
@@ -151,3 +166,22 @@ def ptr(t):
 def stream_ptr():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+class _Here:
+    """A context that changes nothing: the device is the current one already."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_CTX = _Here()
+
+
+def on_device(device):
+    """Makes `device` current for a call (stream_ptr() is the current device's stream)."""
+    import torch
+    return _HERE_CTX if torch.cuda.current_device() == device.index else torch.cuda.device(device)

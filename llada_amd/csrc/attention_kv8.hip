@@ -1,0 +1,496 @@
+// Bidirectional attention over the 8-bit key/value cache (layout: kv8.h), head_dim 128, bf16 queries and output.
+//
+//   out[q] = sum_k p_qk v_k / sum_k p_qk,   p_qk = exp(q . k / sqrt(128) - m_q)
+//
+// over the sequence's unmasked tokens; the tokens of [blk_start, blk_start + blk_len) come from fresh bf16 rows instead
+// of the cache (a block-cached denoise step recomputes them).  A query whose sequence has no unmasked token gets zeros.
+//
+// A wave holds 32 queries and sweeps 64-key tiles: S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_bf16, a query's
+// scores in one lane pair.  Few queries meet each key here, so the sweep is bound by memory and then by the vector pipe,
+// not by the matrix pipe, and the cache's tile order is chosen for that: a wave loads the codes of a tile with sixteen
+// contiguous 1-KiB loads straight into operand registers, the next tile's keys while this tile's softmax and values are
+// worked on and the next tile's values during the next scores; there is no LDS staging and no barrier in the loop.
+// Codes become bf16 exactly (e4m3: one conversion for two codes; int8: three instructions for two); a tile's
+// key scale goes into the multiplier of the scores, its value scale, a power of two 2^e, into the exponent of the
+// probabilities (p 2^e = 2^(s - m + e)), so neither costs an instruction per element.
+//
+// Scores, running maximum, sums and outputs are float32; P is rounded to bf16 once for the matrix unit, like the keys' and
+// values' bf16 forms it multiplies (relative 2^-9 per term, averaged over the terms).
+#include "kv8.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+constexpr int QW = 32;                       // queries of a wave
+constexpr int NWAVES = 4;
+constexpr int OROW = KV8_HD * 4 + 16;        // bytes of a float32 output row in LDS (16 bytes of padding)
+constexpr int SLICE = QW * OROW;             // one wave's LDS: a 64 x 256-byte tile of fresh values, or its result
+static_assert(SLICE >= KV8_TOKENS * 256, "a wave's slice holds a tile of fresh values");
+
+template <int TYPE>
+__device__ __forceinline__ bf16x8 codes_to_bf16(unsigned a, unsigned b) {
+    bf16x8 r;
+    if constexpr (TYPE == LLADA_KV_E4M3) {
+        const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+        const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+        const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+        const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+        r = (bf16x8){x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            r[i] = (__bf16)(float)(signed char)(a >> (8 * i));
+            r[4 + i] = (__bf16)(float)(signed char)(b >> (8 * i));
+        }
+    }
+    return r;
+}
+
+struct Kv8Attn {
+    const bf16_t* q;
+    int64_t q_stride;
+    const float* scales;
+    const unsigned char* tiles;
+    const uint8_t* key_mask;
+    bf16_t* out;
+    const bf16_t* blk;        // fresh [Q | K | V] rows, or null
+    int64_t blk_stride;
+    float* part_o;            // key splits: [split][row][d] float32, unnormalised
+    float* part_ml;           // [split][row][head][2]: running maximum (log2 domain), sum
+    int64_t n_rows;
+    int n_q, seq_len, n_heads, n_blocks, n_qblocks;
+    int blk_start, blk_len;
+    int skip_from, skipped;   // cached tiles [skip_from, skip_from + skipped) lie inside the fresh block
+    int n_cached, n_units;    // tiles to sweep: cached ones, then fresh ones
+    int splits, per_split;
+    float scale_log2e;
+};
+
+// A wave's state over the tiles it has swept.
+struct Softmax {
+    f32x16 o[4];
+    float m, l;
+};
+
+// One tile's scores -> probabilities, the running maximum and sum brought up to date.  s: raw scores (lane: query
+// lane & 31; register 4 c + e of s[kb]: key 32 kb + 8 c + 4 (lane >> 5) + e); valid: bit per key; sc: multiplier into the
+// log2 domain; ve: exponent of the tile's value scale.
+__device__ __forceinline__ void softmax_tile(f32x16 (&s)[2], uint64_t valid, float sc, float ve, float inv_vs, Softmax& w,
+                                             bf16x8 (&pb)[2][2], int hg) {
+    if (valid != ~0ull) {
+        const uint64_t mine = valid >> (4 * hg);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!((mine >> (kb * 32 + 8 * (i >> 2) + (i & 3))) & 1)) s[kb][i] = -INFINITY;   // selected, not added: a masked NaN is gone
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * sc;
+    // the reference maximum moves only when it has risen by more than 2^8: the 64 multiplies of the
+    // accumulators are then rare, and probabilities up to 2^8 are as exact as those below 1
+    const float m_cand = fmaxf(w.m, mx);
+    if (__builtin_amdgcn_ballot_w64(m_cand > w.m + 8.0f) != 0) {
+        const float alpha = __builtin_amdgcn_exp2f(w.m - (m_cand == -INFINITY ? 0.f : m_cand));
+        w.m = m_cand;
+        w.l *= alpha;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w.o[db][e] *= alpha;
+    }
+    const float off = ve - (w.m == -INFINITY ? 0.f : w.m);
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e], sc, off));
+            sum += p;
+            pb[kb][e >> 3][e & 7] = (__bf16)p;
+        }
+    w.l = __builtin_fmaf(sum, inv_vs, w.l);
+}
+
+// NQ query groups of 32 and 4 / NQ key groups per workgroup: few queries -> the waves share the queries and deal the
+// tiles among themselves, their results merged once at the end; many -> each wave has queries of its own and the waves
+// meet a tile's codes in the CU's cache.
+template <int TYPE, int NQ>
+__global__ void __launch_bounds__(NWAVES * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
+    constexpr int NK = NWAVES / NQ;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[NWAVES * SLICE + NWAVES * QW * 8];
+    float* const ml = (float*)(lds + NWAVES * SLICE);       // [wave][query][2]
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, hg = lane >> 5;
+    const int qg = wave % NQ, kg = wave / NQ;
+    // consecutive workgroups go to the 8 XCDs in turn: the query blocks of one head, which read the same
+    // tiles, are made consecutive items of one XCD and meet in its L2
+    int qb, h, b, ks;
+    {
+        const int nt = gridDim.x, bid = blockIdx.x;
+        const int xcd = bid & 7, per = nt >> 3, rem = nt & 7;
+        int item = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (bid >> 3);
+        qb = item % a.n_qblocks;
+        item /= a.n_qblocks;
+        ks = item % a.splits;
+        item /= a.splits;
+        h = item % a.n_heads;
+        b = item / a.n_heads;
+    }
+    const int d = a.n_heads * KV8_HD;
+    const int q0 = (qb * NQ + qg) * QW;
+    const int64_t tile0 = ((int64_t)b * a.n_heads + h) * a.n_blocks;
+    const unsigned char* const tiles = a.tiles + (size_t)tile0 * KV8_TILE + lane * 16;
+    const float* const scales = a.scales + tile0 * 2;
+    const uint8_t* const mask = a.key_mask ? a.key_mask + (size_t)b * a.seq_len : nullptr;
+    const int blk_end = a.blk_start + a.blk_len;
+
+    // lane holds Q[q0 + r][64 hg + 8 i .. + 7]: the contraction runs over the dims in the order of the key codes
+    bf16x8 qf[8];
+    {
+        const int q = min(q0 + r, a.n_q - 1);
+        const bf16_t* qp = a.q + ((size_t)b * a.n_q + q) * (size_t)a.q_stride + h * KV8_HD + hg * 64;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[i] = *(const bf16x8*)(qp + i * 8);
+    }
+    Softmax w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w.o[i][e] = 0.f;
+    w.m = -INFINITY;
+    w.l = 0.f;
+
+    const int u_end = min(a.n_units, (ks + 1) * a.per_split);
+    int u = ks * a.per_split + kg;
+
+    // ---- cached tiles ----
+    auto tile_of = [&](int i) { return i < a.skip_from ? i : i + a.skipped; };
+    u32x4 kc[8], vc[8];
+    auto load_keys = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) kc[i] = *(const u32x4*)(tiles + (size_t)t * KV8_TILE + i * 1024);
+    };
+    auto load_values = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vc[i] = *(const u32x4*)(tiles + (size_t)t * KV8_TILE + KV8_CODES + i * 1024);
+    };
+    // which keys of tile t this kernel takes from the cache
+    auto live_keys = [&](int t, uint8_t m) {
+        const int key = t * KV8_TOKENS + lane;
+        return __builtin_amdgcn_ballot_w64(key < a.seq_len && m != 0 && !(key >= a.blk_start && key < blk_end));
+    };
+    auto mask_byte = [&](int t) -> uint8_t { return mask ? mask[min(t * KV8_TOKENS + lane, a.seq_len - 1)] : (uint8_t)1; };
+
+    const int c_end = min(u_end, a.n_cached);
+    if (u < c_end) {
+        int t = tile_of(u);
+        load_keys(t);
+        load_values(t);
+        uint8_t mb = mask_byte(t);
+        float ks_next = scales[2 * t], vs_next = scales[2 * t + 1];
+        for (; u < c_end; u += NK) {
+            const uint64_t valid = live_keys(t, mb);
+            const float kscale = ks_next, vscale = vs_next;
+            const int tn = u + NK < c_end ? tile_of(u + NK) : t;      // (the last tile is fetched once more and dropped)
+            f32x16 s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+                        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            codes_to_bf16<TYPE>(kc[kb * 4 + j][2 * half], kc[kb * 4 + j][2 * half + 1]), qf[2 * j + half], s[kb], 0, 0, 0);
+            load_keys(tn);
+            mb = mask_byte(tn);
+            ks_next = scales[2 * tn];
+            vs_next = scales[2 * tn + 1];
+            bf16x8 pb[2][2];
+            const float ve = (float)((int)(__float_as_uint(vscale) >> 23) - 127);
+            softmax_tile(s, valid, a.scale_log2e * kscale, ve, __uint_as_float((254u << 23) - __float_as_uint(vscale)), w, pb, hg);
+            if (valid != ~0ull) {          // zero codes under masked keys: 0 * NaN would reach the sums
+                const uint64_t mine = valid >> (4 * hg);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned nib = (unsigned)(mine >> (kb * 32 + 8 * i)) & 15u;
+                        const unsigned keep = ((nib * 0x00204081u) & 0x01010101u) * 255u;
+#pragma unroll
+                        for (int db = 0; db < 4; ++db) vc[db * 2 + kb][i] &= keep;
+                    }
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int ss = 0; ss < 2; ++ss)
+#pragma unroll
+                    for (int db = 0; db < 4; ++db)
+                        w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            codes_to_bf16<TYPE>(vc[db * 2 + kb][2 * ss], vc[db * 2 + kb][2 * ss + 1]), pb[kb][ss], w.o[db], 0, 0, 0);
+            load_values(tn);
+            t = tn;
+        }
+    }
+
+    // ---- fresh tiles: bf16 rows; the values cross the wave's LDS slice to be read transposed ----
+    unsigned char* const slice = lds + wave * SLICE;
+    for (; u < u_end; u += NK) {
+        const int f0 = (u - a.n_cached) * KV8_TOKENS;                   // first row of the tile inside the block
+        const bf16_t* const rows = a.blk + (size_t)b * a.blk_len * (size_t)a.blk_stride + h * KV8_HD + d;
+        const int fk = f0 + lane;
+        const uint8_t fm = mask && fk < a.blk_len ? mask[a.blk_start + fk] : (uint8_t)1;
+        const uint64_t valid = __builtin_amdgcn_ballot_w64(fk < a.blk_len && fm != 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int row = i * 4 + (lane >> 4), c = lane & 15;
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if ((valid >> row) & 1) v = *(const u32x4*)(rows + d + (size_t)(f0 + row) * (size_t)a.blk_stride + c * 8);
+            *(u32x4*)(slice + row * 256 + (((c >> 2) ^ (row & 3)) << 6) + (c & 3) * 16) = v;
+        }
+        f32x16 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+            const bf16_t* kp = rows + (size_t)min(f0 + kb * 32 + r, a.blk_len - 1) * (size_t)a.blk_stride + hg * 64;
+            bf16x8 kf[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) kf[i] = *(const bf16x8*)(kp + i * 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], qf[i], s[kb], 0, 0, 0);
+        }
+        bf16x8 pb[2][2];
+        softmax_tile(s, valid, a.scale_log2e, 0.f, 1.f, w, pb, hg);
+        const int q4 = (lane & 15) >> 2, p4 = lane & 3, g1 = (lane >> 4) & 1;
+        const unsigned char* const vrow = slice + (4 * hg + q4) * 256 + 32 * g1 + 8 * p4;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int ss = 0; ss < 2; ++ss)
+#pragma unroll
+                for (int db = 0; db < 4; ++db) {
+                    const unsigned char* p = vrow + (kb * 32 + 16 * ss) * 256 + ((db * 64) ^ (q4 * 64));
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p);
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 8 * 256));
+                    const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pb[kb][ss], w.o[db], 0, 0, 0);
+                }
+    }
+
+    // ---- the key groups' results, rescaled to their common maximum, are summed out of LDS ----
+    const float l_tot = w.l + __shfl_xor(w.l, 32);
+    if (hg == 0) {
+        ml[(wave * QW + r) * 2] = w.m;
+        ml[(wave * QW + r) * 2 + 1] = l_tot;
+    }
+    __syncthreads();
+    float m_all = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) m_all = fmaxf(m_all, ml[((k * NQ + qg) * QW + r) * 2]);
+    const float f = __builtin_amdgcn_exp2f(w.m - (m_all == -INFINITY ? 0.f : m_all));
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *(f32x4*)(slice + r * OROW + (db * 32 + 8 * c + 4 * hg) * 4) =
+                (f32x4){w.o[db][4 * c] * f, w.o[db][4 * c + 1] * f, w.o[db][4 * c + 2] * f, w.o[db][4 * c + 3] * f};
+    __syncthreads();
+    // wave kg of a query group writes 32 / NK of its queries: 16 lanes a row, 8 dims a lane
+#pragma unroll
+    for (int i = 0; i < QW / NK / 4; ++i) {
+        const int row = kg * (QW / NK) + i * 4 + (lane >> 4), c = lane & 15;
+        float mr = -INFINITY, lr = 0.f;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) mr = fmaxf(mr, ml[((k * NQ + qg) * QW + row) * 2]);
+        const float mu = mr == -INFINITY ? 0.f : mr;
+        f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const int wv = k * NQ + qg;
+            lr += ml[(wv * QW + row) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(wv * QW + row) * 2] - mu);
+            const unsigned char* p = lds + wv * SLICE + row * OROW + c * 32;
+            x0 += *(const f32x4*)p;
+            x1 += *(const f32x4*)(p + 16);
+        }
+        const int q = q0 + row;
+        if (q >= a.n_q) continue;
+        const int64_t orow = (int64_t)b * a.n_q + q;
+        if (a.splits > 1) {
+            float* po = a.part_o + ((size_t)ks * a.n_rows + orow) * d + h * KV8_HD + c * 8;
+            *(f32x4*)po = x0;
+            *(f32x4*)(po + 4) = x1;
+            if (c == 0) {
+                float* pm = a.part_ml + (((size_t)ks * a.n_rows + orow) * a.n_heads + h) * 2;
+                pm[0] = mr;
+                pm[1] = lr;
+            }
+        } else {
+            const float inv = lr == 0.f ? 0.f : 1.0f / lr;              // no unmasked token: zeros
+            u32x4 o;
+            o[0] = pack_bf16x2(x0[0] * inv, x0[1] * inv);
+            o[1] = pack_bf16x2(x0[2] * inv, x0[3] * inv);
+            o[2] = pack_bf16x2(x1[0] * inv, x1[1] * inv);
+            o[3] = pack_bf16x2(x1[2] * inv, x1[3] * inv);
+            *(u32x4*)(a.out + (size_t)orow * d + h * KV8_HD + c * 8) = o;
+        }
+    }
+}
+
+// Key splits: out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, m = max_s m_s; one thread per 4 columns.
+__global__ void __launch_bounds__(256) attn_kv8_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                                                               bf16_t* __restrict__ out, int64_t n_rows, int n_heads, int splits) {
+    const int d = n_heads * KV8_HD;
+    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i >= n_rows * (d / 4)) return;
+    const int64_t row = i / (d / 4);
+    const int col = (int)(i % (d / 4)) * 4, h = col / KV8_HD;
+    float m = -INFINITY;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[((s * n_rows + row) * n_heads + h) * 2]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const float* pm = part_ml + ((s * n_rows + row) * n_heads + h) * 2;
+        const float f = __builtin_amdgcn_exp2f(pm[0] - mu);
+        const f32x4 o = *(const f32x4*)(part_o + (s * n_rows + row) * (int64_t)d + col);
+        l += f * pm[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += f * o[e];
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    u32x2 w;
+    w[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    w[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+    *(u32x2*)(out + row * d + col) = w;
+}
+
+constexpr int MAX_SPLITS = 16;
+
+// Key splits of a launch of `wgs` workgroups over `units` tiles: up to about 512 workgroups (two per CU), none with
+// fewer than two tiles for each of its key groups.
+int pick_splits(int64_t wgs, int units, int nk) {
+    if (wgs >= 256) return 1;
+    int64_t s = 512 / wgs;
+    const int most = units / (2 * nk);
+    s = s < most ? s : most;
+    s = s < MAX_SPLITS ? s : MAX_SPLITS;
+    return s < 1 ? 1 : (int)s;
+}
+
+int query_groups(int n_q) { return n_q <= 32 ? 1 : n_q <= 64 ? 2 : 4; }
+
+size_t part_bytes(int64_t n_rows, int n_heads, int splits) {
+    return (size_t)splits * n_rows * ((size_t)n_heads * KV8_HD * 4 + (size_t)n_heads * 8);
+}
+
+template <int TYPE>
+void launch(const Kv8Attn& a, int nq, unsigned grid, hipStream_t st) {
+    if (nq == 1)
+        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 1>), dim3(grid), dim3(NWAVES * 64), 0, st, a);
+    else if (nq == 2)
+        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 2>), dim3(grid), dim3(NWAVES * 64), 0, st, a);
+    else
+        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 4>), dim3(grid), dim3(NWAVES * 64), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" size_t llada_attn_kv8_workspace_bytes(int32_t n_seq, int32_t n_q, int32_t seq_len, int32_t n_heads) {
+    if (n_seq <= 0 || n_q <= 0 || seq_len <= 0 || n_heads <= 0) return 0;
+    const int nq = query_groups(n_q);
+    const int64_t wgs = (int64_t)((n_q + nq * QW - 1) / (nq * QW)) * n_heads * n_seq;
+    const int splits = pick_splits(wgs, (int)kv8_blocks(seq_len) + 1, NWAVES / nq);     // + 1: a fresh block cut by tile borders
+    return splits > 1 ? part_bytes((int64_t)n_seq * n_q, n_heads, splits) : 0;
+}
+
+extern "C" int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, const void* cache, int32_t kv_type,
+                              const uint8_t* key_mask, void* out, int32_t n_seq, int32_t seq_len, int32_t n_heads,
+                              const void* block_qkv, int64_t block_stride, int32_t block_start, int32_t block_len,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+    LLADA_CHECK_ARG(q && cache && out, "attn_kv8: null argument");
+    LLADA_CHECK_ARG(n_seq > 0 && seq_len > 0 && n_heads > 0 && n_q > 0, "attn_kv8: bad shape");
+    LLADA_CHECK_ARG(q_stride >= (int64_t)n_heads * KV8_HD && q_stride % 8 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0,
+                    "attn_kv8: query rows cover the heads; rows start at 16-byte boundaries");
+    LLADA_CHECK_ARG(((uintptr_t)cache & 255) == 0, "attn_kv8: cache must be 256-byte aligned");
+    LLADA_CHECK_SUPPORTED(kv_type == LLADA_KV_E4M3 || kv_type == LLADA_KV_INT8, "attn_kv8: unknown cache type %d", kv_type);
+    LLADA_CHECK_ARG(workspace == nullptr || ((uintptr_t)workspace & 15) == 0, "attn_kv8: workspace must be 16-byte aligned");
+    if (block_qkv) {
+        LLADA_CHECK_ARG(block_start >= 0 && block_len > 0 && (int64_t)block_start + block_len <= seq_len,
+                        "attn_kv8: the block must lie inside the sequence");
+        LLADA_CHECK_ARG(block_stride >= (int64_t)3 * n_heads * KV8_HD && block_stride % 8 == 0 && ((uintptr_t)block_qkv & 15) == 0,
+                        "attn_kv8: block rows hold [Q | K | V] and start at 16-byte boundaries");
+    }
+    const int64_t n_blocks = kv8_blocks(seq_len);
+    const int64_t n_tiles = (int64_t)n_seq * n_heads * n_blocks;
+    Kv8Attn a;
+    a.q = (const bf16_t*)q;
+    a.q_stride = q_stride;
+    a.scales = (const float*)cache;
+    a.tiles = (const unsigned char*)cache + kv8_scale_bytes(n_tiles);
+    a.key_mask = key_mask;
+    a.out = (bf16_t*)out;
+    a.blk = (const bf16_t*)block_qkv;
+    a.blk_stride = block_stride;
+    a.n_rows = (int64_t)n_seq * n_q;
+    a.n_q = n_q;
+    a.seq_len = seq_len;
+    a.n_heads = n_heads;
+    a.n_blocks = (int)n_blocks;
+    a.scale_log2e = 1.4426950408889634f / sqrtf((float)KV8_HD);
+    a.blk_start = block_qkv ? block_start : 0;
+    a.blk_len = block_qkv ? block_len : 0;
+    a.skip_from = (int)n_blocks;
+    a.skipped = 0;
+    int fresh = 0;
+    if (block_qkv) {
+        const int end = block_start + block_len;
+        const int c0 = (block_start + KV8_TOKENS - 1) / KV8_TOKENS, c1 = end == seq_len ? (int)n_blocks : end / KV8_TOKENS;
+        if (c1 > c0) {
+            a.skip_from = c0;
+            a.skipped = c1 - c0;
+        }
+        fresh = (block_len + KV8_TOKENS - 1) / KV8_TOKENS;
+    }
+    a.n_cached = (int)n_blocks - a.skipped;
+    a.n_units = a.n_cached + fresh;
+    const int nq = query_groups(n_q);
+    a.n_qblocks = (n_q + nq * QW - 1) / (nq * QW);
+    const int64_t wgs = (int64_t)a.n_qblocks * n_heads * n_seq;
+    int splits = workspace ? pick_splits(wgs, a.n_units, NWAVES / nq) : 1;
+    while (splits > 1 && part_bytes(a.n_rows, n_heads, splits) > workspace_bytes) --splits;
+    a.per_split = (a.n_units + splits - 1) / splits;
+    a.splits = (a.n_units + a.per_split - 1) / a.per_split;             // no empty run
+    a.part_o = (float*)workspace;
+    a.part_ml = a.splits > 1 ? a.part_o + (size_t)a.splits * a.n_rows * n_heads * KV8_HD : nullptr;
+    LLADA_CHECK_SUPPORTED(wgs * a.splits < 0x7fffffffLL && a.n_rows * n_heads * (KV8_HD / 4) / 256 < 0x7fffffffLL,
+                          "attn_kv8: grid too large");
+    hipStream_t st = (hipStream_t)stream;
+    if (kv_type == LLADA_KV_E4M3)
+        launch<LLADA_KV_E4M3>(a, nq, (unsigned)(wgs * a.splits), st);
+    else
+        launch<LLADA_KV_INT8>(a, nq, (unsigned)(wgs * a.splits), st);
+    LLADA_CHECK_LAUNCH("attn_kv8_kernel");
+    if (a.splits > 1) {
+        const int64_t items = a.n_rows * n_heads * (KV8_HD / 4);
+        hipLaunchKernelGGL(attn_kv8_combine_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st,
+                           (const float*)a.part_o, (const float*)a.part_ml, a.out, a.n_rows, n_heads, a.splits);
+        LLADA_CHECK_LAUNCH("attn_kv8_combine_kernel");
+    }
+    return LLADA_OK;
+}

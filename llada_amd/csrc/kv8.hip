@@ -1,0 +1,267 @@
+// Writing and reading the 8-bit key/value cache (layout: kv8.h).
+//
+// Each 64-token block of a head is held as 8-bit codes times one power of two: scale = 2^k with the smallest k for
+// which the block's largest magnitude fits the code's range (448 for e4m3, 127 for int8), code = round to nearest
+// even of x * 2^-k.  Power-of-two scales make x * 2^-k exact (the only rounding is the one to the code), make every
+// stored value exact in bf16, and let the attention kernel fold a scale into an exponent.  They cost e4m3 nothing
+// (its steps are relative) and int8 at most one of its eight bits.
+//
+// Masked tokens are stored as zeros and do not enter the scale, so padding cannot coarsen its block; infinities
+// saturate and do not enter the scale either; a NaN stays a NaN in e4m3 and becomes 0 in int8, which has none.
+#include "kv8.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+// exponent k of a block's scale
+template <int TYPE>
+__device__ __forceinline__ int scale_exponent(float amax) {
+    if (amax == 0.f) return 0;
+    const unsigned u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127;
+    const unsigned frac = u & 0x7FFFFFu;
+    // 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6
+    const int k = TYPE == LLADA_KV_E4M3 ? e - 8 + (frac > 0x600000u) : e - 6 + (frac > 0x7E0000u);
+    return k < -126 ? -126 : k;          // keeps the scale and its inverse normal numbers
+}
+
+__device__ __forceinline__ float power_of_two(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }
+
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? a : 0.f;
+}
+
+// four values -> four codes
+template <int TYPE>
+__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv) {
+    float y[4] = {a * inv, b * inv, c * inv, d * inv};
+    if constexpr (TYPE == LLADA_KV_E4M3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = y[i] != y[i] ? y[i] : __builtin_amdgcn_fmed3f(y[i], -448.f, 448.f);
+        int r = 0;
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], r, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
+        return (unsigned)r;
+    } else {
+        unsigned r = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = y[i] != y[i] ? 0 : (int)__builtin_rintf(__builtin_amdgcn_fmed3f(y[i], -127.f, 127.f));
+            r |= (unsigned)(v & 255) << (8 * i);
+        }
+        return r;
+    }
+}
+
+template <int TYPE>
+__device__ __forceinline__ float decode(unsigned word, int byte) {
+    if constexpr (TYPE == LLADA_KV_E4M3) {
+        switch (byte) {
+            case 0: return __builtin_amdgcn_cvt_f32_fp8((int)word, 0);
+            case 1: return __builtin_amdgcn_cvt_f32_fp8((int)word, 1);
+            case 2: return __builtin_amdgcn_cvt_f32_fp8((int)word, 2);
+            default: return __builtin_amdgcn_cvt_f32_fp8((int)word, 3);
+        }
+    } else {
+        return (float)(signed char)(word >> (8 * byte));
+    }
+}
+
+// One workgroup = one (sequence, head, block): thread (kg, dg) holds keys 4 kg .. + 3 and dims 8 dg .. + 7 of the keys
+// and of the values (two whole 256-byte head rows per four threads of loads).  Bound by memory: 4 bytes in and 2 out
+// per channel; the codes cross the LDS once to leave as whole 1-KiB runs.
+template <int TYPE>
+__global__ void __launch_bounds__(THREADS) kv8_write_kernel(const bf16_t* __restrict__ rows, int64_t row_stride,
+                                                            const uint8_t* __restrict__ key_mask, float* __restrict__ scales,
+                                                            unsigned char* __restrict__ tiles, int seq_len, int n_heads,
+                                                            int n_blocks, int start, int len, int first_block,
+                                                            int touched) {
+    __shared__ __attribute__((aligned(16))) unsigned char codes[KV8_TILE];
+    __shared__ float red[2][THREADS / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int kg = tid >> 4, dg = tid & 15;
+    int64_t item = blockIdx.x;
+    const int h = (int)(item % n_heads);
+    item /= n_heads;
+    const int t = first_block + (int)(item % touched);
+    const int b = (int)(item / touched);
+    const int64_t tile = ((int64_t)b * n_heads + h) * n_blocks + t;
+    unsigned char* const dst = tiles + (size_t)tile * KV8_TILE;
+    float* const sc = scales + tile * 2;
+    const int d = n_heads * KV8_HD;
+    const int key0 = t * KV8_TOKENS + kg * 4;
+
+    float x[2][4][8];                    // keys, values
+    bool old[4];                         // a token outside the range that stays: taken as the cache holds it
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int key = key0 + i;
+        const bool live = key < seq_len && (key_mask == nullptr || key_mask[(size_t)b * seq_len + key] != 0);
+        const bool fresh = key >= start && key < start + len;
+        old[i] = live && !fresh;
+        u32x4 w[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+        if (live && fresh) {
+            const bf16_t* p = rows + ((size_t)b * len + (key - start)) * row_stride + d + h * KV8_HD + dg * 8;
+            w[0] = *(const u32x4*)p;
+            w[1] = *(const u32x4*)(p + d);
+        }
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[o][i][e] = __uint_as_float((e & 1) ? (w[o][e >> 1] & 0xFFFF0000u) : (w[o][e >> 1] << 16));
+    }
+    // a block that the range covers only in part: its other tokens as the cache holds them (uniform branch)
+    const int t_end = min(seq_len, (t + 1) * KV8_TOKENS);
+    if (start > t * KV8_TOKENS || start + len < t_end) {
+        const float sk = sc[0], sv = sc[1];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned vw = *(const unsigned*)(dst + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (old[i]) x[1][i][e] = decode<TYPE>(vw, i) * sv;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (old[i]) {
+                const u32x2 kw = *(const u32x2*)(dst + kv8_key_offset(kg * 4 + i, dg * 8));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[0][i][e] = decode<TYPE>(kw[e >> 2], e & 3) * sk;
+            }
+        }
+    }
+
+    float amax[2] = {0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax[o] = fmaxf(amax[o], finite_abs(x[o][i][e]));
+        amax[o] = wave_reduce_max(amax[o]);
+        if (lane == 0) red[o][wave] = amax[o];
+    }
+    __syncthreads();                     // also: every old code of this tile has been read
+    int k[2];
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+        float m = red[o][0];
+#pragma unroll
+        for (int w = 1; w < THREADS / 64; ++w) m = fmaxf(m, red[o][w]);
+        k[o] = scale_exponent<TYPE>(m);
+    }
+    const float ik = power_of_two(-k[0]), iv = power_of_two(-k[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        u32x2 w;
+        w[0] = encode4<TYPE>(x[0][i][0], x[0][i][1], x[0][i][2], x[0][i][3], ik);
+        w[1] = encode4<TYPE>(x[0][i][4], x[0][i][5], x[0][i][6], x[0][i][7], ik);
+        *(u32x2*)(codes + kv8_key_offset(kg * 4 + i, dg * 8)) = w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        *(unsigned*)(codes + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e)) =
+            encode4<TYPE>(x[1][0][e], x[1][1][e], x[1][2][e], x[1][3][e], iv);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < KV8_TILE / (16 * THREADS); ++i) {
+        const int at = (i * THREADS + tid) * 16;
+        *(u32x4*)(dst + at) = *(const u32x4*)(codes + at);
+    }
+    if (tid < 2) sc[tid] = power_of_two(k[tid]);
+}
+
+// The values a layer of the cache stands for, as bf16 rows (exact: at most seven significant bits times a power of two).
+template <int TYPE>
+__global__ void __launch_bounds__(THREADS) kv8_read_kernel(const float* __restrict__ scales,
+                                                           const unsigned char* __restrict__ tiles, bf16_t* __restrict__ k_out,
+                                                           bf16_t* __restrict__ v_out, int seq_len, int n_heads, int n_blocks) {
+    __shared__ __attribute__((aligned(16))) unsigned char codes[KV8_TILE];
+    const int tid = threadIdx.x, kg = tid >> 4, dg = tid & 15;
+    int64_t item = blockIdx.x;
+    const int h = (int)(item % n_heads);
+    item /= n_heads;
+    const int t = (int)(item % n_blocks);
+    const int b = (int)(item / n_blocks);
+    const int64_t tile = ((int64_t)b * n_heads + h) * n_blocks + t;
+    const unsigned char* const src = tiles + (size_t)tile * KV8_TILE;
+    const float sk = scales[tile * 2], sv = scales[tile * 2 + 1];
+#pragma unroll
+    for (int i = 0; i < KV8_TILE / (16 * THREADS); ++i) {
+        const int at = (i * THREADS + tid) * 16;
+        *(u32x4*)(codes + at) = *(const u32x4*)(src + at);
+    }
+    __syncthreads();
+    unsigned vw[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vw[e] = *(const unsigned*)(codes + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int key = t * KV8_TOKENS + kg * 4 + i;
+        if (key >= seq_len) continue;
+        const u32x2 kw = *(const u32x2*)(codes + kv8_key_offset(kg * 4 + i, dg * 8));
+        u32x4 a, c;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            a[w] = pack_bf16x2(decode<TYPE>(kw[w >> 1], (2 * w) & 3) * sk, decode<TYPE>(kw[w >> 1], (2 * w + 1) & 3) * sk);
+            c[w] = pack_bf16x2(decode<TYPE>(vw[2 * w], i) * sv, decode<TYPE>(vw[2 * w + 1], i) * sv);
+        }
+        const size_t at = ((size_t)b * seq_len + key) * ((size_t)n_heads * KV8_HD) + (size_t)h * KV8_HD + dg * 8;
+        *(u32x4*)(k_out + at) = a;
+        *(u32x4*)(v_out + at) = c;
+    }
+}
+
+}  // namespace
+
+extern "C" size_t llada_kv8_layer_bytes(int32_t n_seq, int32_t seq_len, int32_t n_heads) {
+    if (n_seq <= 0 || seq_len <= 0 || n_heads <= 0) return 0;
+    const int64_t n_tiles = (int64_t)n_seq * n_heads * kv8_blocks(seq_len);
+    return kv8_scale_bytes(n_tiles) + (size_t)n_tiles * KV8_TILE;
+}
+
+extern "C" int llada_kv8_write(const void* qkv, int64_t row_stride, const uint8_t* key_mask, void* cache, int32_t kv_type,
+                               int32_t n_seq, int32_t seq_len, int32_t n_heads, int32_t start, int32_t len, void* stream) {
+    LLADA_CHECK_ARG(qkv && cache, "kv8_write: null argument");
+    LLADA_CHECK_ARG(n_seq > 0 && seq_len > 0 && n_heads > 0, "kv8_write: bad shape");
+    LLADA_CHECK_ARG(start >= 0 && len > 0 && (int64_t)start + len <= seq_len, "kv8_write: rows %d .. %lld of %d", start,
+                    (long long)start + len, seq_len);
+    LLADA_CHECK_ARG(row_stride >= (int64_t)3 * n_heads * KV8_HD && row_stride % 8 == 0 && ((uintptr_t)qkv & 15) == 0,
+                    "kv8_write: rows hold [Q | K | V] and start at 16-byte boundaries");
+    LLADA_CHECK_ARG(((uintptr_t)cache & 255) == 0, "kv8_write: cache must be 256-byte aligned");
+    LLADA_CHECK_SUPPORTED(kv_type == LLADA_KV_E4M3 || kv_type == LLADA_KV_INT8, "kv8_write: unknown cache type %d", kv_type);
+    const int64_t n_blocks = kv8_blocks(seq_len);
+    const int64_t n_tiles = (int64_t)n_seq * n_heads * n_blocks;
+    const int first = start / KV8_TOKENS, touched = (start + len - 1) / KV8_TOKENS - first + 1;
+    const int64_t grid = (int64_t)n_seq * n_heads * touched;
+    LLADA_CHECK_SUPPORTED(grid < 0x7fffffffLL, "kv8_write: grid too large");
+    float* scales = (float*)cache;
+    unsigned char* tiles = (unsigned char*)cache + kv8_scale_bytes(n_tiles);
+    auto kernel = kv_type == LLADA_KV_E4M3 ? kv8_write_kernel<LLADA_KV_E4M3> : kv8_write_kernel<LLADA_KV_INT8>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), 0, (hipStream_t)stream, (const bf16_t*)qkv, row_stride,
+                       key_mask, scales, tiles, seq_len, n_heads, (int)n_blocks, start, len, first, touched);
+    LLADA_CHECK_LAUNCH("kv8_write_kernel");
+    return LLADA_OK;
+}
+
+extern "C" int llada_kv8_read(const void* cache, int32_t kv_type, void* k_out, void* v_out, int32_t n_seq, int32_t seq_len,
+                              int32_t n_heads, void* stream) {
+    LLADA_CHECK_ARG(cache && k_out && v_out, "kv8_read: null argument");
+    LLADA_CHECK_ARG(n_seq > 0 && seq_len > 0 && n_heads > 0, "kv8_read: bad shape");
+    LLADA_CHECK_ARG(((uintptr_t)cache & 255) == 0 && (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0,
+                    "kv8_read: cache must be 256-byte, outputs 16-byte aligned");
+    LLADA_CHECK_SUPPORTED(kv_type == LLADA_KV_E4M3 || kv_type == LLADA_KV_INT8, "kv8_read: unknown cache type %d", kv_type);
+    const int64_t n_blocks = kv8_blocks(seq_len);
+    const int64_t n_tiles = (int64_t)n_seq * n_heads * n_blocks;
+    LLADA_CHECK_SUPPORTED(n_tiles < 0x7fffffffLL, "kv8_read: grid too large");
+    const float* scales = (const float*)cache;
+    const unsigned char* tiles = (const unsigned char*)cache + kv8_scale_bytes(n_tiles);
+    auto kernel = kv_type == LLADA_KV_E4M3 ? kv8_read_kernel<LLADA_KV_E4M3> : kv8_read_kernel<LLADA_KV_INT8>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n_tiles), dim3(THREADS), 0, (hipStream_t)stream, scales, tiles, (bf16_t*)k_out,
+                       (bf16_t*)v_out, seq_len, n_heads, (int)n_blocks);
+    LLADA_CHECK_LAUNCH("kv8_read_kernel");
+    return LLADA_OK;
+}

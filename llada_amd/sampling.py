@@ -1,0 +1,75 @@
+"""Truncated sampling: temperature, top-k, top-p and min-p from one given uniform per row.
+
+The reference's temperature (generate.py:8-19) is a Gumbel-max over the whole vocabulary and offers no truncation; this
+is the operator behind ``generate(top_k=, top_p=, min_p=)``, for callers that sample rows of logits themselves."""
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+
+def truncates(temperature, top_k, top_p, min_p):
+    """Whether these scalars draw from a truncated distribution (temperature 0 is the arg-max whatever they are)."""
+    return temperature != 0 and (top_k > 0 or top_p < 1.0 or min_p > 0.0)
+
+
+def scalar_sampling(temperature, top_k, top_p, min_p, uniforms=None):
+    """The C parameters for one value of each; ``uniforms``: float64 tensor, or None for the library's own stream."""
+    return _lib.Sampling(float(temperature), float(top_p), float(min_p), int(top_k), None, None, None, None, _lib.ptr(uniforms))
+
+
+def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uniforms=None, uncond_logits=None, cfg_scale=0.0,
+                  seed=0, step=0, row_offset=0, return_probs=False):
+    """One token id per row of ``logits`` [..., vocab] (bf16), int64 [...].
+
+    With a row's entries ordered by (logit descending, index ascending) and w_i = exp((l_i - max) / temperature) in
+    float64: top-k keeps the first ``top_k`` (0: all), top-p the shortest prefix of those with at least ``top_p`` of
+    their mass, min-p the entries with w_i >= ``min_p``; what all three keep (at least one entry) is sampled: the token is
+    the first whose running mass exceeds u times the kept total.  temperature 0 gives the arg-max.  ``temperature``,
+    ``top_k``, ``top_p`` and ``min_p`` may each be a tensor with one value per row.
+
+    ``uniforms`` [...] float64 in [0, 1); without it u comes from the library's Philox stream, counters (row, step) with
+    the rows numbered from ``row_offset``.  ``uncond_logits`` (same shape): combined with ``cfg_scale`` first, as
+    generate.py:89-90 does.  ``return_probs``: also the tokens' probabilities among the kept entries (float32)."""
+    if logits.dtype != torch.bfloat16 or not logits.is_cuda or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits: a bfloat16 GPU tensor [..., vocab] is wanted")
+    lib, dev = _lib.load(), logits.device
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    n = rows.shape[0]
+    if rows.stride(1) != 1 and vocab > 1 or (n > 1 and rows.stride(0) < vocab):
+        rows = rows.contiguous()
+    stride = rows.stride(0) if n > 1 else vocab
+    un = None
+    if uncond_logits is not None:
+        if uncond_logits.shape != logits.shape or uncond_logits.dtype != torch.bfloat16 or uncond_logits.device != dev:
+            raise ValueError("uncond_logits: the shape, type and device of logits are wanted")
+        un = uncond_logits.reshape(-1, vocab)
+        if un.stride() != rows.stride():
+            rows, un, stride = rows.contiguous(), un.contiguous(), vocab
+    keep = []
+
+    def per_row(v, dtype):
+        if not isinstance(v, torch.Tensor):
+            return None
+        if v.dim() and v.shape != lead:
+            raise ValueError(f"a sampling parameter has shape {list(v.shape)}, the rows {list(lead)}")
+        keep.append(v.to(device=dev, dtype=dtype).expand(lead).reshape(-1).contiguous())
+        return keep[-1].data_ptr()
+
+    arrays = [per_row(temperature, torch.float32), per_row(top_k, torch.int32), per_row(top_p, torch.float32), per_row(min_p, torch.float32)]
+    t, k, p, q = (d if a is not None else v for v, d, a in zip((temperature, top_k, top_p, min_p), (1.0, 0, 1.0, 0.0), arrays))
+    u = None
+    if uniforms is not None:
+        if uniforms.shape != lead or uniforms.device != dev:
+            raise ValueError(f"uniforms: shape {list(lead)} on {dev} is wanted")
+        u = uniforms.to(torch.float64).reshape(-1).contiguous()
+    with _lib.on_device(dev):
+        tokens = torch.empty(lead, dtype=torch.int64, device=dev)
+        probs = torch.empty(lead, dtype=torch.float32, device=dev) if return_probs else None
+        if n:
+            s = _lib.Sampling(float(t), float(p), float(q), int(k), *arrays, _lib.ptr(u))
+            _lib.check(lib.llada_sample_rows(rows.data_ptr(), _lib.ptr(un), stride, float(cfg_scale), n, vocab, C.byref(s), seed, step,
+                                             row_offset, tokens.data_ptr(), _lib.ptr(probs), _lib.stream_ptr()))
+    return (tokens, probs) if return_probs else tokens

@@ -1,0 +1,324 @@
+"""The 8-bit key/value cache and the attention over it on an MI355X, against float64 restatements (oracle/kv8.py).
+
+Written values are exact (power-of-two scales: the only rounding is the code's own), so the cache is compared bit for
+bit.  Attention: the probabilities are rounded to bf16 once (2^-8 relative: half a step) before they are summed with the
+values, the result once more; scores carry the float32 error of 128 products, at most 130 * 2^-24 of |q| |k|, and the
+exponential's argument a rounding of its own size, below 2^-19 for scores up to 32 in the log2 domain.  A relative error e
+of the scores' exponent moves numerator and denominator by e each, hence
+    |out - exact| <= 2^-8 (spread + |exact|) + 2 e spread + 2^-20 spread,   spread = sum p |v| / sum p."""
+import numpy as np
+import pytest
+
+from oracle import kv8 as okv
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def rows(seed, n, L, H, poison=None):
+    """bf16 [Q | K | V] rows with uneven key channels; poison: positions whose keys and values hold NaN / inf."""
+    g = np.random.Generator(np.random.PCG64(seed))
+    x = g.standard_normal((n, L, 3, H, 128)).astype(np.float32)
+    x[:, :, 1] *= np.exp(0.7 * g.standard_normal((H, 128))).astype(np.float32)
+    if poison is not None:
+        for b, t, val in poison:
+            x[b, t, 1:] = val
+    return torch.from_numpy(x.reshape(n, L, 3 * H * 128)).cuda().to(torch.bfloat16)
+
+
+def split(x, H):
+    n, L, _ = x.shape
+    y = x.double().cpu().numpy().reshape(n, L, 3, H, 128)
+    return y[:, :, 0], y[:, :, 1], y[:, :, 2]
+
+
+def values(cache, layer=0):
+    return [t.double().cpu().numpy() for t in cache.read(layer)]
+
+
+def make(n, L, H, dtype, layers=1):
+    from llada_amd import KVCache8
+    return KVCache8(n, L, H, n_layers=layers, dtype=dtype, device="cuda")
+
+
+def left_mask(n, L, seed=0):
+    g = np.random.Generator(np.random.PCG64(seed + 91))
+    m = np.ones((n, L), dtype=np.uint8)
+    for b in range(n):
+        m[b, :int(g.integers(0, max(1, L // 2 + 1)))] = 0
+    return m
+
+
+def same(a, b):
+    return np.array_equal(a, b, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("n,L,H,masked", [(1, 1, 1, False), (2, 63, 2, True), (1, 64, 3, False), (2, 65, 2, False), (3, 200, 5, True)])
+def test_fill_is_exact(lib, n, L, H, masked, dtype):
+    x = rows(L + H, n, L, H)
+    m = left_mask(n, L) if masked else None
+    c = make(n, L, H, dtype)
+    c.fill(0, x, None if m is None else torch.from_numpy(m).cuda())
+    _, k, v = split(x, H)
+    gk, gv = values(c)
+    assert same(gk, okv.held(k, dtype, m)) and same(gv, okv.held(v, dtype, m))
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+def test_fill_values_of_every_size(lib, dtype):
+    """Scale borders (largest magnitude at the code's range times a power of two and one step past it), subnormal codes,
+    zeros, infinities, NaN, the smallest and largest bf16 values."""
+    L, H = 64 * 6, 2
+    x = rows(5, 1, L, H).float().reshape(1, L, 3, H, 128)
+    x[0, 0:64] *= 2.0 ** -9
+    x[0, 7, 1, 0, 3], x[0, 7, 2, 0, 3] = 448.0, 127.0
+    x[0, 64:128] = 0.0
+    x[0, 70, 1, 1, 0] = 450.0
+    x[0, 71, 2, 1, 0] = 127.5
+    x[0, 128:192] *= 1e-30
+    x[0, 192:256] *= 2.0 ** 100
+    x[0, 200, 1, 0, 5] = float("inf")
+    x[0, 201, 2, 0, 5] = float("-inf")
+    x[0, 202, 1, 1, 9] = float("nan")
+    x[0, 203, 2, 1, 9] = float("nan")
+    x[0, 256:320] *= 2.0 ** -100
+    x[0, 330, 1, 0, :] = -0.0
+    xb = x.reshape(1, L, -1).to(torch.bfloat16)
+    c = make(1, L, H, dtype)
+    c.fill(0, xb)
+    _, k, v = split(xb, H)
+    gk, gv = values(c)
+    assert same(gk, okv.held(k, dtype)) and same(gv, okv.held(v, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("L,start,length", [(200, 0, 200), (200, 70, 1), (200, 64, 64), (200, 60, 10), (200, 137, 63), (200, 199, 1),
+                                            (65, 0, 64), (300, 10, 250)])
+def test_update_requantises_the_touched_blocks(lib, L, start, length, dtype):
+    n, H = 2, 3
+    m = left_mask(n, L, 7)
+    mt = torch.from_numpy(m).cuda()
+    x, y = rows(1, n, L, H), rows(2, n, length, H) * 3
+    c = make(n, L, H, dtype, layers=3)
+    c.fill(1, x, mt)
+    c.update(1, y, start, mt)
+    _, k, v = split(x, H)
+    _, yk, yv = split(y, H)
+    gk, gv = values(c, 1)
+    assert same(gk, okv.updated(okv.held(k, dtype, m), yk, start, dtype, m))
+    assert same(gv, okv.updated(okv.held(v, dtype, m), yv, start, dtype, m))
+    for other in (0, 2):                       # the neighbouring layers stay what they were: zeros
+        for t in values(c, other):
+            assert not t.any()
+
+
+def test_update_of_a_fresh_cache(lib):
+    """A block of a new cache that is written in part holds zeros elsewhere."""
+    c = make(1, 100, 2, "e4m3")
+    y = rows(3, 1, 7, 2)
+    c.update(0, y, 61)
+    _, yk, _ = split(y, 2)
+    want = okv.updated(np.zeros((1, 100, 2, 128)), yk, 61, "e4m3")
+    assert same(values(c)[0], want)
+
+
+def test_strided_and_flat_rows(lib):
+    n, L, H = 2, 70, 2
+    x = rows(4, n, L, H)
+    want = None
+    wide = torch.zeros((n, L, 3 * H * 128 + 64), dtype=torch.bfloat16, device="cuda")
+    wide[..., :3 * H * 128] = x
+    odd = torch.zeros((n, L, 3 * H * 128 + 3), dtype=torch.bfloat16, device="cuda")
+    odd[..., :3 * H * 128] = x
+    bigger = torch.zeros((n, L + 9, 3 * H * 128), dtype=torch.bfloat16, device="cuda")
+    bigger[:, 4:4 + L] = x
+    shifted = torch.zeros(x.numel() + 1, dtype=torch.bfloat16, device="cuda")[1:].view(x.shape)
+    shifted.copy_(x)
+    for form in (x, x.reshape(n * L, -1), wide, odd, bigger[:, 4:4 + L], shifted, x.transpose(0, 1).contiguous().transpose(0, 1)):
+        c = make(n, L, H, "int8")
+        c.fill(0, form)
+        got = values(c)
+        out = c.attend(0, form[:, 5:15] if form.dim() == 3 else x[:, 5:15]).float().cpu().numpy()
+        want = want or (got, out)
+        assert same(got[0], want[0][0]) and same(got[1], want[0][1]) and same(out, want[1])
+
+
+def check_attend(c, x, H, n_q, dtype, m, fresh, start, fresh_rows=None):
+    n, L, d = x.shape[0], x.shape[1], H * 128
+    y = rows(77 + n_q, n, n_q, H) if fresh_rows is None else fresh_rows
+    mt = None if m is None else torch.from_numpy(m).cuda()
+    c.fill(0, x, mt)
+    out = c.attend(0, y, mt, block=y if fresh else None, block_start=start if fresh else 0)
+    assert out.shape == (n, n_q, d) and out.dtype == torch.bfloat16
+    _, k, v = split(x, H)
+    k, v = okv.held(k, dtype, m), okv.held(v, dtype, m)
+    q, yk, yv = split(y, H)
+    if fresh:
+        k[:, start:start + n_q], v[:, start:start + n_q] = yk, yv
+    want, spread = okv.attend(q, k, v, m)
+    got = out.double().cpu().numpy().reshape(n, n_q, H, 128)
+    keep = np.ones((n, L), bool) if m is None else m.astype(bool)
+    kn = np.sqrt((np.where(keep[:, :, None, None], k, 0.0) ** 2).sum(-1)).max() if keep.any() else 0.0
+    e = 130 * 2.0 ** -24 * np.sqrt((q ** 2).sum(-1)).max() * kn / np.sqrt(128) + 2.0 ** -19
+    tol = 2.0 ** -8 * (spread + np.abs(want)) + (2 * e + 2.0 ** -20) * spread
+    assert np.isfinite(got).all()
+    worst = np.max(np.abs(got - want) - tol)
+    assert worst <= 0, f"beyond the bound by {worst:.3g} (largest bound {tol.max():.3g})"
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("n,L,H,n_q,start,fresh", [
+    (1, 1, 1, 1, 0, False), (1, 1, 1, 1, 0, True), (2, 64, 2, 1, 63, True), (1, 65, 3, 31, 10, True), (2, 200, 2, 32, 60, True),
+    (1, 384, 2, 33, 320, True), (3, 130, 1, 64, 64, True), (1, 257, 2, 65, 0, True), (2, 300, 2, 129, 171, True), (1, 200, 2, 200, 0, True),
+    (1, 1030, 1, 32, 512, True), (2, 1030, 1, 200, 830, True), (1, 2100, 2, 3, 0, False), (1, 700, 5, 300, 0, False)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attend(lib, n, L, H, n_q, start, fresh, masked, dtype):
+    m = left_mask(n, L, n_q) if masked else None
+    check_attend(make(n, L, H, dtype), rows(L, n, L, H), H, n_q, dtype, m, fresh, start)
+
+
+@pytest.mark.parametrize("n_q", [1, 40, 100])
+def test_rows_a_mask_leaves_empty_and_poisoned_padding(lib, n_q):
+    """One sequence without any unmasked token gives zeros; NaN and infinities under masked tokens, cached or fresh, reach
+    nothing."""
+    n, L, H, start = 3, 200, 2, 90
+    m = np.ones((n, L), dtype=np.uint8)
+    m[0] = 0
+    m[1, :70] = 0
+    m[1, 90] = 0
+    m[2, 150:] = 0
+    bad = [(1, 3, float("nan")), (1, 64, float("inf")), (2, 199, float("-inf")), (0, 5, float("nan"))]
+    x = rows(8, n, L, H, bad)
+    y = rows(9, n, n_q, H)
+    y.view(n, n_q, 3, H, 128)[1, 0, 1:] = float("nan")
+    y.view(n, n_q, 3, H, 128)[0, 0, 1:] = float("inf")
+    c = make(n, L, H, "e4m3")
+    out = check_attend(c, x, H, n_q, "e4m3", m, True, start, y)
+    assert not out[0].any()
+
+
+def test_cached_nan_under_a_later_mask(lib):
+    """A NaN that the cache holds (written unmasked) does not reach the result of a call that masks its token; a call that
+    attends it gives NaN."""
+    n, L, H = 1, 130, 1
+    x = rows(12, n, L, H, [(0, 77, float("nan"))])
+    c = make(n, L, H, "e4m3")
+    c.fill(0, x)
+    m = torch.ones((n, L), dtype=torch.uint8, device="cuda")
+    m[0, 77] = 0
+    y = rows(13, n, 4, H)
+    assert torch.isfinite(c.attend(0, y, m)).all()
+    assert torch.isnan(c.attend(0, y)).all()
+
+
+def test_one_hot_and_uniform(lib):
+    """A query that matches one key only returns that key's value; equal scores return the mean."""
+    L, H = 300, 2
+    x = torch.zeros((1, L, 3, H, 128), dtype=torch.bfloat16, device="cuda")
+    g = np.random.Generator(np.random.PCG64(5))
+    x[0, :, 2] = torch.from_numpy(g.integers(-8, 9, size=(L, H, 128)).astype(np.float32)).cuda().to(torch.bfloat16)
+    x[0, :, 1, :, 0] = -100.0
+    x[0, 217, 1, :, 0] = 100.0
+    c = make(1, L, H, "int8")
+    c.fill(0, x.view(1, L, -1))
+    q = torch.zeros((1, 3, 3, H, 128), dtype=torch.bfloat16, device="cuda")
+    q[0, 1, 0, :, 0] = 64.0
+    out = c.attend(0, q.view(1, 3, -1)).view(3, H, 128)
+    assert torch.equal(out[1], x[0, 217, 2])
+    mean = x[0, :, 2].double().mean(0)
+    assert ((out[0].double() - mean).abs() <= 2.0 ** -8 * mean.abs() + 1e-6).all()       # p = 1 exactly: only the output rounds
+
+
+def test_masks_of_every_type(lib):
+    n, L, H = 2, 90, 1
+    m = left_mask(n, L, 3)
+    x, y = rows(14, n, L, H), rows(15, n, 5, H)
+    ref = None
+    for t in (torch.from_numpy(m).cuda(), torch.from_numpy(m).cuda().bool(), torch.from_numpy(m).cuda().long() * 7,
+              torch.from_numpy(m).cuda().float(), torch.from_numpy(np.ascontiguousarray(m.T)).cuda().T):
+        c = make(n, L, H, "e4m3")
+        c.fill(0, x, t)
+        out = c.attend(0, y, t)
+        ref = out if ref is None else ref
+        assert torch.equal(out, ref)
+
+
+def test_key_splits_and_neighbours(lib):
+    """The same rows with and without the key splits' scratch agree to rounding, and a query's result does not depend on the
+    other sequences of the call."""
+    n, L, H, n_q = 2, 3000, 2, 32
+    x, y = rows(20, n, L, H), rows(21, n, n_q, H)
+    c = make(n, L, H, "e4m3")
+    c.fill(0, x)
+    assert lib.llada_attn_kv8_workspace_bytes(n, n_q, L, H) > 0
+    a = c.attend(0, y)
+    c._ws_bytes[n_q] = 0
+    b = c.attend(0, y)
+    assert (a.float() - b.float()).abs().max() <= 2.0 ** -6 * a.float().abs().max()
+    one = make(1, L, H, "e4m3")
+    one.fill(0, x[1:])
+    one._ws_bytes[n_q] = 0
+    assert torch.equal(one.attend(0, y[1:]), b[1:])
+
+
+def test_outputs_past_the_rows_stay(lib):
+    n, L, H, n_q = 1, 100, 2, 5
+    c = make(n, L, H, "e4m3")
+    c.fill(0, rows(22, n, L, H))
+    buf = torch.full((n * n_q + 4, H * 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = buf[:n * n_q].view(n, n_q, H * 128)
+    y = rows(23, n, n_q, H)
+    assert torch.equal(c.attend(0, y, out=out), c.attend(0, y))
+    assert (buf[n * n_q:] == 7.0).all()
+    with pytest.raises(ValueError):
+        c.attend(0, y, out=buf)
+
+
+def test_refusals(lib):
+    from llada_amd import KVCache8
+    c = make(2, 100, 2, "e4m3")
+    x = rows(24, 2, 100, 2)
+    for call in (lambda: c.fill(0, x[:1]), lambda: c.fill(0, x.float()), lambda: c.fill(0, x[..., :700]), lambda: c.update(0, x, 1),
+                 lambda: c.update(0, x[:, :5], -1), lambda: c.update(0, x[:, :5].reshape(10, -1), 0), lambda: c.fill(0, x, torch.ones(2, 99, device="cuda")),
+                 lambda: c.fill(0, x, torch.ones(2, 100)), lambda: c.attend(0, x[:, :5], block=x[:, :5], block_start=96),
+                 lambda: c.attend(0, x[:, :0]), lambda: c.attend(0, x[0, :5]), lambda: c.fill(0, x.cpu())):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(IndexError):
+        c.fill(1, x)
+    with pytest.raises(IndexError):
+        c.read(-1)
+    with pytest.raises(NotImplementedError):
+        KVCache8(1, 1, 1, dtype="bf16")
+
+
+def test_captured_step_on_a_side_stream(lib):
+    """update + attend captured once and replayed with new inputs, eager calls on the same cache in between, against eager
+    results each time."""
+    n, L, H, n_q, start = 2, 700, 2, 32, 300
+    c, e = make(n, L, H, "int8"), make(n, L, H, "int8")
+    x = rows(30, n, L, H)
+    c.fill(0, x)
+    e.fill(0, x)
+    buf = rows(31, n, n_q, H)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.attend(0, buf, block=buf, block_start=start)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = c.attend(0, buf, block=buf, block_start=start)
+            c.update(0, buf, start)
+            after = c.read(0)
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        buf.copy_(rows(40 + i, n, n_q, H))
+        g.replay()
+        want = e.attend(0, buf, block=buf, block_start=start)
+        e.update(0, buf, start)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(after[0], e.read(0)[0]) and torch.equal(after[1], e.read(0)[1])
+        torch.cuda.synchronize()
