@@ -269,6 +269,20 @@ int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, const void* cac
                    int32_t block_start, int32_t block_len, void* workspace, size_t workspace_bytes, void* stream);
 size_t llada_attn_kv8_workspace_bytes(int32_t n_seq, int32_t n_q, int32_t seq_len, int32_t n_heads);
 
+/* llada_forward_fill_cache / llada_forward_block over such caches, one a layer, in order (kv_cache: llada_kv8_bytes bytes,
+ * 256-byte aligned).  The filling step's logits are llada_forward's; a block's step attends its own rows in bf16 and the
+ * rest as the cache holds it, and with update_cache the block's rows are written afterwards. */
+size_t llada_kv8_bytes(const llada_config* cfg, int32_t n_seq, int32_t seq_len);
+int llada_forward_fill_cache_kv8(const llada_config* cfg, const llada_weights* w, const int64_t* ids,
+                                 const uint8_t* key_mask, const float* rope_cos, const float* rope_sin, int32_t n_seq,
+                                 int32_t seq_len, const int32_t* logit_rows, int32_t n_logit_rows, void* logits_out,
+                                 void* workspace, size_t workspace_bytes, void* kv_cache, int32_t kv_type, void* stream);
+int llada_forward_block_kv8(const llada_config* cfg, const llada_weights* w, const int64_t* block_ids,
+                            const uint8_t* key_mask, const float* rope_cos, const float* rope_sin, int32_t n_seq,
+                            int32_t seq_len, int32_t block_start, int32_t block_len, void* kv_cache, int32_t kv_type,
+                            int32_t update_cache, const int32_t* logit_rows, int32_t n_logit_rows, void* logits_out,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Sampler epilogue: replaces generate.py:81-134 after the forward.
  * ------------------------------------------------------------------------------------------- */

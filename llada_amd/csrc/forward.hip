@@ -79,7 +79,9 @@ __global__ void __launch_bounds__(256) scatter_kv_kernel(const bf16_t* __restric
 int forward_impl(const llada_config* cfg, const llada_weights* w, const int64_t* ids, const uint8_t* key_mask,
                  const float* rope_cos, const float* rope_sin, int32_t n_seq, int32_t seq_len,
                  const int32_t* logit_rows, int32_t n_logit_rows, void* logits_out, void* workspace,
-                 size_t workspace_bytes, void* kv_cache, const int32_t* positions, void* stream);
+                 size_t workspace_bytes, void* kv_cache, int32_t kv_type, const int32_t* positions, void* stream);
+
+constexpr int32_t KV_IMAGE = -1;   // kv_type of a cache that is the bf16 [Q | K | V] image itself
 
 }  // namespace
 
@@ -89,7 +91,7 @@ extern "C" int llada_forward_positions(const llada_config* cfg, const llada_weig
                                        int32_t n_logit_rows, void* logits_out, void* workspace, size_t workspace_bytes,
                                        void* stream) {
     return forward_impl(cfg, w, ids, key_mask, rope_cos, rope_sin, n_seq, seq_len, logit_rows, n_logit_rows, logits_out,
-                        workspace, workspace_bytes, nullptr, positions, stream);
+                        workspace, workspace_bytes, nullptr, KV_IMAGE, positions, stream);
 }
 
 extern "C" int llada_forward(const llada_config* cfg, const llada_weights* w, const int64_t* ids,
@@ -97,7 +99,7 @@ extern "C" int llada_forward(const llada_config* cfg, const llada_weights* w, co
                              int32_t seq_len, const int32_t* logit_rows, int32_t n_logit_rows, void* logits_out,
                              void* workspace, size_t workspace_bytes, void* stream) {
     return forward_impl(cfg, w, ids, key_mask, rope_cos, rope_sin, n_seq, seq_len, logit_rows, n_logit_rows, logits_out,
-                        workspace, workspace_bytes, nullptr, nullptr, stream);
+                        workspace, workspace_bytes, nullptr, KV_IMAGE, nullptr, stream);
 }
 
 extern "C" size_t llada_kv_cache_bytes(const llada_config* cfg, int32_t n_seq, int32_t seq_len) {
@@ -112,7 +114,22 @@ extern "C" int llada_forward_fill_cache(const llada_config* cfg, const llada_wei
                                         void* stream) {
     LLADA_CHECK_ARG(kv_cache != nullptr && ((uintptr_t)kv_cache & 255) == 0, "forward_fill_cache: kv_cache must be 256-byte aligned");
     return forward_impl(cfg, w, ids, key_mask, rope_cos, rope_sin, n_seq, seq_len, logit_rows, n_logit_rows, logits_out,
-                        workspace, workspace_bytes, kv_cache, nullptr, stream);
+                        workspace, workspace_bytes, kv_cache, KV_IMAGE, nullptr, stream);
+}
+
+extern "C" size_t llada_kv8_bytes(const llada_config* cfg, int32_t n_seq, int32_t seq_len) {
+    return cfg && cfg->n_layers > 0 ? (size_t)cfg->n_layers * llada_kv8_layer_bytes(n_seq, seq_len, cfg->n_heads) : 0;
+}
+
+extern "C" int llada_forward_fill_cache_kv8(const llada_config* cfg, const llada_weights* w, const int64_t* ids,
+                                            const uint8_t* key_mask, const float* rope_cos, const float* rope_sin,
+                                            int32_t n_seq, int32_t seq_len, const int32_t* logit_rows, int32_t n_logit_rows,
+                                            void* logits_out, void* workspace, size_t workspace_bytes, void* kv_cache,
+                                            int32_t kv_type, void* stream) {
+    LLADA_CHECK_ARG(kv_cache != nullptr && ((uintptr_t)kv_cache & 255) == 0, "forward_fill_cache_kv8: kv_cache must be 256-byte aligned");
+    LLADA_CHECK_SUPPORTED(kv_type == LLADA_KV_E4M3 || kv_type == LLADA_KV_INT8, "forward_fill_cache_kv8: unknown cache type %d", kv_type);
+    return forward_impl(cfg, w, ids, key_mask, rope_cos, rope_sin, n_seq, seq_len, logit_rows, n_logit_rows, logits_out,
+                        workspace, workspace_bytes, kv_cache, kv_type, nullptr, stream);
 }
 
 namespace {
@@ -120,7 +137,7 @@ namespace {
 int forward_impl(const llada_config* cfg, const llada_weights* w, const int64_t* ids, const uint8_t* key_mask,
                  const float* rope_cos, const float* rope_sin, int32_t n_seq, int32_t seq_len,
                  const int32_t* logit_rows, int32_t n_logit_rows, void* logits_out, void* workspace,
-                 size_t workspace_bytes, void* kv_cache, const int32_t* positions, void* stream) {
+                 size_t workspace_bytes, void* kv_cache, int32_t kv_type, const int32_t* positions, void* stream) {
     LLADA_CHECK_ARG(cfg && w && ids && rope_cos && rope_sin && logits_out && workspace, "forward: null argument");
     LLADA_CHECK_ARG(n_seq > 0 && seq_len > 0 && n_logit_rows > 0, "forward: bad shape");
     const llada_config& c = *cfg;
@@ -165,8 +182,8 @@ int forward_impl(const llada_config* cfg, const llada_weights* w, const int64_t*
     bool final_norm_done = false;
     for (int l = 0; l < c.n_layers; ++l) {
         const bool last = l == c.n_layers - 1;
-        // with a cache every layer leaves its [Q | K | V] image there instead of in the shared scratch
-        if (kv_cache) qkv = (unsigned char*)kv_cache + (size_t)l * M * 3 * d * 2;
+        // with an image cache every layer leaves its [Q | K | V] image there instead of in the shared scratch
+        if (kv_cache && kv_type == KV_IMAGE) qkv = (unsigned char*)kv_cache + (size_t)l * M * 3 * d * 2;
         if (w->packed & 1) {
             TRY(llada_gemm_bf16_positions(h, w->wqkv[l], qkv, M, 3 * d, d, d, 3 * d, LLADA_EPI_ROPE_QKV | tf, nullptr, 0,
                                           rope_cos, rope_sin, seq_len, positions, sk, skb, stream));
@@ -176,6 +193,9 @@ int forward_impl(const llada_config* cfg, const llada_weights* w, const int64_t*
             TRY(llada_rope_bf16_positions(qkv, rope_cos, rope_sin, n_seq, seq_len, c.n_heads, positions, stream));
         }
         TRY(llada_attn_bidir_bf16(qkv, key_mask, att, n_seq, seq_len, c.n_heads, stream));
+        if (kv_cache && kv_type != KV_IMAGE)      // this step attends the rows as they are; later steps what the cache holds
+            TRY(llada_kv8_write(qkv, (int64_t)3 * d, key_mask, (unsigned char*)kv_cache + (size_t)l * llada_kv8_layer_bytes(n_seq, seq_len, c.n_heads),
+                                kv_type, n_seq, seq_len, c.n_heads, 0, seq_len, stream));
         int64_t Ml = M;      // rows from here to the end of the layer
         void* xl = x;        // residual stream of those rows
         void* al = att;      // attention output of those rows
@@ -222,14 +242,15 @@ int forward_impl(const llada_config* cfg, const llada_weights* w, const int64_t*
 
 }  // namespace
 
+namespace {
+
 // One denoising step of the block-cached sampler: only the block_len positions starting at block_start of
 // every sequence are recomputed (block_ids [n_seq, block_len]); their keys and values replace the cached ones
 // and their queries attend over the whole cached sequence.  logits_out [n_seq * block_len, vocab].
-extern "C" int llada_forward_block(const llada_config* cfg, const llada_weights* w, const int64_t* block_ids,
-                                   const uint8_t* key_mask, const float* rope_cos, const float* rope_sin, int32_t n_seq,
-                                   int32_t seq_len, int32_t block_start, int32_t block_len, void* kv_cache,
-                                   int32_t update_cache, const int32_t* logit_rows, int32_t n_logit_rows,
-                                   void* logits_out, void* workspace, size_t workspace_bytes, void* stream) {
+int block_impl(const llada_config* cfg, const llada_weights* w, const int64_t* block_ids, const uint8_t* key_mask,
+               const float* rope_cos, const float* rope_sin, int32_t n_seq, int32_t seq_len, int32_t block_start,
+               int32_t block_len, void* kv_cache, int32_t kv_type, int32_t update_cache, const int32_t* logit_rows,
+               int32_t n_logit_rows, void* logits_out, void* workspace, size_t workspace_bytes, void* stream) {
     LLADA_CHECK_ARG(cfg && w && block_ids && rope_cos && rope_sin && logits_out && workspace && kv_cache,
                     "forward_block: null argument");
     LLADA_CHECK_ARG(logit_rows == nullptr || n_logit_rows > 0, "forward_block: logit_rows without a count");
@@ -242,7 +263,8 @@ extern "C" int llada_forward_block(const llada_config* cfg, const llada_weights*
     const int64_t Mb = (int64_t)n_seq * block_len;
     const int64_t M = (int64_t)n_seq * seq_len;
     const Layout lay = make_layout(c, Mb, Mb);
-    const size_t attn_bytes = llada_attn_workspace_bytes(n_seq, block_len, seq_len, c.n_heads);   // key-split partials
+    const size_t attn_bytes = kv_type == KV_IMAGE ? llada_attn_workspace_bytes(n_seq, block_len, seq_len, c.n_heads)   // key-split partials
+                                                  : llada_attn_kv8_workspace_bytes(n_seq, block_len, seq_len, c.n_heads);
     if (workspace_bytes < lay.total + attn_bytes) {
         llada_set_error("forward_block: workspace has %zu bytes, %zu needed", workspace_bytes, lay.total + attn_bytes);
         return LLADA_ERR_WORKSPACE;
@@ -270,7 +292,9 @@ extern "C" int llada_forward_block(const llada_config* cfg, const llada_weights*
     if (c.n_layers > 0) TRY(llada_rmsnorm_bf16(x, w->attn_norm[0], h, Mb, d, c.rms_eps, nullptr, stream));
     for (int l = 0; l < c.n_layers; ++l) {
         const bool last = l == c.n_layers - 1;
-        bf16_t* image = (bf16_t*)((unsigned char*)kv_cache + (size_t)l * M * 3 * d * 2);
+        const size_t layer_bytes = kv_type == KV_IMAGE ? (size_t)M * 3 * d * 2 : llada_kv8_layer_bytes(n_seq, seq_len, c.n_heads);
+        void* const layer = (unsigned char*)kv_cache + (size_t)l * layer_bytes;
+        bf16_t* image = (bf16_t*)layer;
         if (w->packed & 1) {
             TRY(llada_gemm_bf16(h, w->wqkv[l], qkv, Mb, 3 * d, d, d, 3 * d, LLADA_EPI_ROPE_QKV | tf, nullptr, 0, cos_b, sin_b,
                                 block_len, sk, skb, stream));
@@ -279,15 +303,22 @@ extern "C" int llada_forward_block(const llada_config* cfg, const llada_weights*
                                 0, sk, skb, stream));
             TRY(llada_rope_bf16(qkv, cos_b, sin_b, n_seq, block_len, c.n_heads, stream));
         }
-        if (update_cache) {
+        if (update_cache && kv_type == KV_IMAGE) {
             const int64_t total = Mb * (2 * d / 8);
             const int grid = (int)((total + 255) / 256 < 4096 ? (total + 255) / 256 : 4096);
             hipLaunchKernelGGL(scatter_kv_kernel, dim3(grid), dim3(256), 0, st, (const bf16_t*)qkv, image, Mb, block_len,
                                seq_len, block_start, d);
             LLADA_CHECK_LAUNCH("scatter_kv_kernel");
         }
-        TRY(llada_attn_bidir_queries_bf16(qkv, (int64_t)3 * d, block_len, image, key_mask, att, n_seq, seq_len, c.n_heads,
-                                          update_cache ? nullptr : qkv, block_start, attn_ws, attn_bytes, stream));
+        if (kv_type == KV_IMAGE) {
+            TRY(llada_attn_bidir_queries_bf16(qkv, (int64_t)3 * d, block_len, image, key_mask, att, n_seq, seq_len, c.n_heads,
+                                              update_cache ? nullptr : qkv, block_start, attn_ws, attn_bytes, stream));
+        } else {                                  // the block's own rows are attended as they are, written afterwards
+            TRY(llada_attn_kv8(qkv, (int64_t)3 * d, block_len, layer, kv_type, key_mask, att, n_seq, seq_len, c.n_heads, qkv,
+                               (int64_t)3 * d, block_start, block_len, attn_ws, attn_bytes, stream));
+            if (update_cache)
+                TRY(llada_kv8_write(qkv, (int64_t)3 * d, key_mask, layer, kv_type, n_seq, seq_len, c.n_heads, block_start, block_len, stream));
+        }
         TRY(llada_gemm_residual_rmsnorm_bf16(att, w->wo[l], x, h, w->ff_norm[l], c.rms_eps, Mb, d, d, d, tl, sk, skb, stream));
         if (w->packed & 1) {
             TRY(llada_gemm_bf16(h, w->wgu[l], act, Mb, 2 * F, d, d, F, LLADA_EPI_SWIGLU | tf, nullptr, 0, nullptr, nullptr, 0,
@@ -312,9 +343,33 @@ extern "C" int llada_forward_block(const llada_config* cfg, const llada_weights*
     return LLADA_OK;
 }
 
+}  // namespace
+
+extern "C" int llada_forward_block(const llada_config* cfg, const llada_weights* w, const int64_t* block_ids,
+                                   const uint8_t* key_mask, const float* rope_cos, const float* rope_sin, int32_t n_seq,
+                                   int32_t seq_len, int32_t block_start, int32_t block_len, void* kv_cache,
+                                   int32_t update_cache, const int32_t* logit_rows, int32_t n_logit_rows,
+                                   void* logits_out, void* workspace, size_t workspace_bytes, void* stream) {
+    return block_impl(cfg, w, block_ids, key_mask, rope_cos, rope_sin, n_seq, seq_len, block_start, block_len, kv_cache, KV_IMAGE,
+                      update_cache, logit_rows, n_logit_rows, logits_out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int llada_forward_block_kv8(const llada_config* cfg, const llada_weights* w, const int64_t* block_ids,
+                                       const uint8_t* key_mask, const float* rope_cos, const float* rope_sin, int32_t n_seq,
+                                       int32_t seq_len, int32_t block_start, int32_t block_len, void* kv_cache, int32_t kv_type,
+                                       int32_t update_cache, const int32_t* logit_rows, int32_t n_logit_rows,
+                                       void* logits_out, void* workspace, size_t workspace_bytes, void* stream) {
+    LLADA_CHECK_SUPPORTED(kv_type == LLADA_KV_E4M3 || kv_type == LLADA_KV_INT8, "forward_block_kv8: unknown cache type %d", kv_type);
+    return block_impl(cfg, w, block_ids, key_mask, rope_cos, rope_sin, n_seq, seq_len, block_start, block_len, kv_cache, kv_type,
+                      update_cache, logit_rows, n_logit_rows, logits_out, workspace, workspace_bytes, stream);
+}
+
 extern "C" size_t llada_forward_block_workspace_bytes(const llada_config* cfg, int32_t n_seq, int32_t seq_len,
                                                       int32_t block_len) {
     if (!cfg || n_seq <= 0 || block_len <= 0 || seq_len <= 0) return 0;
     const int64_t Mb = (int64_t)n_seq * block_len;
-    return make_layout(*cfg, Mb, Mb).total + llada_attn_workspace_bytes(n_seq, block_len, seq_len, cfg->n_heads);
+    // room for either kind of cache
+    const size_t image = llada_attn_workspace_bytes(n_seq, block_len, seq_len, cfg->n_heads);
+    const size_t kv8 = llada_attn_kv8_workspace_bytes(n_seq, block_len, seq_len, cfg->n_heads);
+    return make_layout(*cfg, Mb, Mb).total + (image > kv8 ? image : kv8);
 }

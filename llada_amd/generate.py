@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 from .model import LLaDAModel, check_token_ids, positions_from_mask
+from .sampling import scalar_sampling, truncates
 
 EOS_ID = 126081   # generate.py:95,101
 EOT_ID = 126348   # generate.py:101
@@ -55,7 +56,7 @@ def get_num_transfer_tokens(mask_index, steps):
 def generate(model, prompt, attention_mask=None, steps=128, gen_length=128, block_length=128, temperature=0.,
              cfg_scale=0., remasking='low_confidence', mask_id=126336, logits_eos_inf=False,
              confidence_eos_eot_inf=False, *, seed=0, row_offset=0, noise_fn=None, rand_fn=None,
-             step_callback=None, cache=None, position_ids=None):
+             step_callback=None, cache=None, position_ids=None, kv_dtype=None, top_k=0, top_p=1.0, min_p=0.0, uniform_fn=None):
     '''
     Args (generate.py:46-59):
         model: Mask predictor (llada_amd.LLaDAModel, or any object with .device and
@@ -87,6 +88,14 @@ def generate(model, prompt, attention_mask=None, steps=128, gen_length=128, bloc
             tiling): what lets a caller batch requests the reference runs one at a time
             (eval_llada.py:260-265) and still get their batch-1 answers.  A [B, P + gen_length] integer
             tensor gives the positions directly.
+        kv_dtype: None (default) keeps the cached keys and values in bf16; "e4m3" or "int8" holds them in 8 bits
+            with a scale for each 64 tokens and head (KVCache8: a third of the memory), a further APPROXIMATION of
+            the cached modes; needs ``cache``.
+        top_k, top_p, min_p: with a temperature, draw each step's candidates from the distribution truncated so
+            (sample_tokens; off by default) instead of the reference's Gumbel-max over the whole vocabulary; the
+            remasking confidence stays the rule on the whole softmax.
+        uniform_fn(shape) -> float64 tensor [B, L] in [0, 1): the draws' uniforms (with a temperature; given
+            without a truncation, it draws from the whole vocabulary by inversion).
     '''
     lib = _lib.load()
     device = torch.device(model.device)
@@ -113,6 +122,11 @@ def generate(model, prompt, attention_mask=None, steps=128, gen_length=128, bloc
         raise NotImplementedError(f"cache={cache!r}")
     if cache is not None and not fast:
         raise NotImplementedError(f"cache={cache!r} needs an llada_amd.LLaDAModel")
+    if kv_dtype is not None and (cache is None or kv_dtype not in _lib.KV_TYPES):
+        raise NotImplementedError(f"kv_dtype={kv_dtype!r} with cache={cache!r}")
+    sampled = truncates(temperature, top_k, top_p, min_p) or (temperature != 0 and uniform_fn is not None)
+    if sampled and noise_fn is not None:
+        raise NotImplementedError("noise_fn is the Gumbel-max's: a truncated draw takes uniform_fn")
     pos = None
     if position_ids is not None:
         if not fast or cache is not None:
@@ -128,7 +142,7 @@ def generate(model, prompt, attention_mask=None, steps=128, gen_length=128, bloc
         if cfg_scale > 0.0:
             pos = torch.cat([pos, pos], dim=0)
         pos = pos.contiguous()
-    kv = model.kv_cache(2 * B if cfg_scale > 0.0 else B, L) if cache is not None else None
+    kv = model.kv_cache(2 * B if cfg_scale > 0.0 else B, L, kv_dtype) if cache is not None else None
     V = model.cfg.vocab_size if fast else None
     x0 = torch.empty_like(x)
     conf = torch.empty((B, L), dtype=torch.float32, device=device)
@@ -215,7 +229,15 @@ def generate(model, prompt, attention_mask=None, steps=128, gen_length=128, bloc
                                    x.data_ptr(), B, L, be, mask_id, _lib.REMASK[remasking], flags, EOS_ID, EOT_ID,
                                    float(temperature), _lib.ptr(noise), _lib.ptr(rand_scores), seed, gstep,
                                    row_offset, x0.data_ptr(), conf.data_ptr(), ws.data_ptr(), ws.numel())
-            _lib.check(lib.llada_remask_scores(C.byref(args), stream))                    # :94-128
+            if sampled:
+                u = None
+                if uniform_fn is not None:
+                    u = uniform_fn((B, L)).to(device=device, dtype=torch.float64).contiguous()
+                    assert tuple(u.shape) == (B, L)
+                sp = scalar_sampling(temperature, top_k, top_p, min_p, u)
+                _lib.check(lib.llada_remask_scores_sampled(C.byref(args), C.byref(sp), stream))
+            else:
+                _lib.check(lib.llada_remask_scores(C.byref(args), stream))                # :94-128
             _lib.check(lib.llada_topk_transfer(x.data_ptr(), x0.data_ptr(), conf.data_ptr(), B, L,
                                                sched.data_ptr(), steps, i, stream))       # :130-134
             if step_callback is not None:

@@ -8,6 +8,7 @@ import ctypes as C
 import torch
 
 from . import _lib
+from .kv_cache import KVCache8
 from .weights import LLaDAConfig, LLaDAWeights
 
 
@@ -100,10 +101,19 @@ class LLaDAModel:
     def _workspace(self, n_seq, L, n_rows):
         return self._scratch("_ws", self.lib.llada_forward_workspace_bytes(C.byref(self._c_cfg), n_seq, L, n_rows))
 
-    def kv_cache(self, n_seq, L):
-        """Storage for the block-cached sampler: every layer's [Q | K | V] image of n_seq x L tokens."""
+    def kv_cache(self, n_seq, L, kv_dtype=None):
+        """Storage for the block-cached sampler: every layer's [Q | K | V] image of n_seq x L tokens (bf16), or with
+        ``kv_dtype`` "e4m3" / "int8" every layer's keys and values in 8 bits (KVCache8, a third of the memory)."""
+        if kv_dtype is not None:
+            return KVCache8(n_seq, L, self.cfg.n_heads, self.cfg.n_layers, kv_dtype, self.device)
         need = self.lib.llada_kv_cache_bytes(C.byref(self._c_cfg), n_seq, L)
         return torch.empty(need, dtype=torch.uint8, device=self.device)
+
+    def _check_kv8(self, kv_cache, n_seq, L):
+        """A KVCache8 is addressed by its own sizes: they have to be this call's."""
+        have = (kv_cache.n_layers, kv_cache.n_seq, kv_cache.seq_len, kv_cache.n_heads)
+        if have != (self.cfg.n_layers, n_seq, L, self.cfg.n_heads) or kv_cache.device != self.weights.wte.device:
+            raise ValueError(f"kv_cache of (layers, sequences, tokens, heads) {have}: {(self.cfg.n_layers, n_seq, L, self.cfg.n_heads)} is wanted")
 
     def forward_block(self, block_ids, attention_mask, seq_len, block_start, kv_cache, out=None, update_cache=True,
                       logit_rows=None):
@@ -120,7 +130,11 @@ class LLaDAModel:
         if attention_mask is not None:
             km = (attention_mask.to(self.device) != 0).to(torch.uint8).contiguous()
             assert tuple(km.shape) == (n_seq, seq_len)
-        assert kv_cache.numel() >= self.lib.llada_kv_cache_bytes(C.byref(self._c_cfg), n_seq, seq_len)
+        kv8 = isinstance(kv_cache, KVCache8)
+        if kv8:
+            self._check_kv8(kv_cache, n_seq, seq_len)
+        else:
+            assert kv_cache.numel() >= self.lib.llada_kv_cache_bytes(C.byref(self._c_cfg), n_seq, seq_len)
         cos, sin = self.rope_tables(seq_len)
         n_rows = n_seq * bl if logit_rows is None else int(logit_rows.numel())
         if logit_rows is not None:
@@ -128,18 +142,20 @@ class LLaDAModel:
         if out is None:
             out = torch.empty(n_rows, self.cfg.vocab_size, dtype=torch.bfloat16, device=self.device)
         ws = self._scratch("_ws_block", self.lib.llada_forward_block_workspace_bytes(C.byref(self._c_cfg), n_seq, seq_len, bl))
-        _lib.check(self.lib.llada_forward_block(C.byref(self._c_cfg), C.byref(self._c_w), ids.data_ptr(), _lib.ptr(km),
-                                                cos.data_ptr(), sin.data_ptr(), n_seq, seq_len, block_start, bl,
-                                                kv_cache.data_ptr(), 1 if update_cache else 0, _lib.ptr(logit_rows),
-                                                n_rows if logit_rows is not None else 0, out.data_ptr(),
-                                                ws.data_ptr(), ws.numel(),
-                                                _lib.stream_ptr()))
+        tail = (1 if update_cache else 0, _lib.ptr(logit_rows), n_rows if logit_rows is not None else 0, out.data_ptr(),
+                ws.data_ptr(), ws.numel(), _lib.stream_ptr())
+        head = (C.byref(self._c_cfg), C.byref(self._c_w), ids.data_ptr(), _lib.ptr(km), cos.data_ptr(), sin.data_ptr(), n_seq,
+                seq_len, block_start, bl)
+        if kv8:
+            _lib.check(self.lib.llada_forward_block_kv8(*head, kv_cache.data.data_ptr(), _lib.KV_TYPES[kv_cache.dtype], *tail))
+        else:
+            _lib.check(self.lib.llada_forward_block(*head, kv_cache.data_ptr(), *tail))
         return out
 
     def forward_rows(self, input_ids, attention_mask=None, logit_rows=None, out=None, kv_cache=None, position_ids=None):
         """Forward on ids [n_seq, L]; returns bf16 logits [n_rows, V] for the flat token indices in
         ``logit_rows`` (int32 tensor) or for every token when it is None.  With ``kv_cache`` every layer's
-        [Q | K | V] image is left there for forward_block.  ``position_ids`` [n_seq, L] (int): the rotary position
+        [Q | K | V] image (a KVCache8: its keys and values in 8 bits) is left there for forward_block.  ``position_ids`` [n_seq, L] (int): the rotary position
         of every token instead of its column index (see positions_from_mask); not together with ``kv_cache``."""
         assert input_ids.dim() == 2 and input_ids.dtype == torch.long
         ids = input_ids.to(self.device).contiguous()
@@ -168,6 +184,12 @@ class LLaDAModel:
             rc = self.lib.llada_forward(C.byref(self._c_cfg), C.byref(self._c_w), ids.data_ptr(), _lib.ptr(km),
                                         cos.data_ptr(), sin.data_ptr(), n_seq, L, _lib.ptr(logit_rows), n_rows,
                                         out.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_ptr())
+        elif isinstance(kv_cache, KVCache8):
+            self._check_kv8(kv_cache, n_seq, L)
+            rc = self.lib.llada_forward_fill_cache_kv8(C.byref(self._c_cfg), C.byref(self._c_w), ids.data_ptr(), _lib.ptr(km),
+                                                       cos.data_ptr(), sin.data_ptr(), n_seq, L, _lib.ptr(logit_rows), n_rows,
+                                                       out.data_ptr(), ws.data_ptr(), ws.numel(), kv_cache.data.data_ptr(),
+                                                       _lib.KV_TYPES[kv_cache.dtype], _lib.stream_ptr())
         else:
             assert kv_cache.numel() >= self.lib.llada_kv_cache_bytes(C.byref(self._c_cfg), n_seq, L)
             rc = self.lib.llada_forward_fill_cache(C.byref(self._c_cfg), C.byref(self._c_w), ids.data_ptr(), _lib.ptr(km),

@@ -11,6 +11,7 @@ from . import _lib
 
 def truncates(temperature, top_k, top_p, min_p):
     """Whether these scalars draw from a truncated distribution (temperature 0 is the arg-max whatever they are)."""
+    assert top_k >= 0 and 0.0 < top_p <= 1.0 and 0.0 <= min_p <= 1.0, f"top_k={top_k}, top_p={top_p}, min_p={min_p}"
     return temperature != 0 and (top_k > 0 or top_p < 1.0 or min_p > 0.0)
 
 

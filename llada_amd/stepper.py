@@ -15,12 +15,13 @@ import torch
 from . import _lib
 from .generate import EOS_ID, EOT_ID
 from .model import LLaDAModel, check_token_ids
+from .sampling import scalar_sampling, truncates
 
 
 class GenerationStepper:
     def __init__(self, model, prompt, attention_mask=None, gen_length=128, block_length=32, temperature=0.,
                  cfg_scale=0., remasking='low_confidence', mask_id=126336, logits_eos_inf=False,
-                 confidence_eos_eot_inf=False, seed=0, max_history=None):
+                 confidence_eos_eot_inf=False, seed=0, max_history=None, top_k=0, top_p=1.0, min_p=0.0):
         assert gen_length % block_length == 0                                             # generate.py:68
         if remasking not in _lib.REMASK:
             raise NotImplementedError(remasking)                                          # :122-123
@@ -36,6 +37,8 @@ class GenerationStepper:
         self.block_length, self.num_blocks = block_length, gen_length // block_length
         self.temperature, self.cfg_scale, self.remasking = float(temperature), float(cfg_scale), remasking
         self.mask_id, self.seed = mask_id, seed
+        # generate()'s truncated draw of the candidates (None: the Gumbel-max, or the arg-max at temperature 0)
+        self.sampling = scalar_sampling(temperature, top_k, top_p, min_p) if truncates(temperature, top_k, top_p, min_p) else None
         self.flags = (_lib.FLAG_LOGITS_EOS_INF if logits_eos_inf else 0) | (_lib.FLAG_CONF_EOS_EOT_INF if confidence_eos_eot_inf else 0)
         self.x = torch.full((B, self.L), mask_id, dtype=torch.long, device=self.device)   # :60-61
         self.x[:, :P] = prompt.to(self.device)
@@ -141,7 +144,10 @@ class GenerationStepper:
                                B, L, be, self.mask_id, _lib.REMASK[self.remasking], self.flags, EOS_ID, EOT_ID,
                                self.temperature, None, None, self.seed, self.step_index, 0, self.x0.data_ptr(),
                                self.conf.data_ptr(), self.ws.data_ptr(), self.ws.numel())
-        _lib.check(self.lib.llada_remask_scores(C.byref(args), _lib.stream_ptr()))        # :94-128
+        if self.sampling is not None:
+            _lib.check(self.lib.llada_remask_scores_sampled(C.byref(args), C.byref(self.sampling), _lib.stream_ptr()))
+        else:
+            _lib.check(self.lib.llada_remask_scores(C.byref(args), _lib.stream_ptr()))    # :94-128
         self.step_index += 1
         self.scores_valid = True
         return self.x0, self.conf

@@ -68,3 +68,12 @@ def test_python_refusals():
     from llada_amd import sample_tokens
     with pytest.raises(ValueError):
         sample_tokens(torch.zeros(2, 8, dtype=torch.bfloat16))              # no GPU tensor
+
+
+@pytest.mark.parametrize("bad", [dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5), dict(top_p=float("nan")), dict(min_p=-0.5), dict(min_p=1.5)])
+def test_scalars_out_of_range_are_refused_even_when_unused(bad):
+    from llada_amd.sampling import truncates
+    ok = dict(top_k=0, top_p=1.0, min_p=0.0)
+    assert not truncates(0.7, **ok) and truncates(0.7, 5, 1.0, 0.0) and not truncates(0, 5, 0.5, 0.1)
+    with pytest.raises(AssertionError):
+        truncates(0, **{**ok, **bad})
