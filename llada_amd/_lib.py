@@ -168,9 +168,11 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def stream_ptr():
+def stream_ptr(device_index=None):
+    """The current stream of a device (default: the current device) as a raw pointer.  Asked of torch's binding directly:
+    making a torch.cuda.Stream object for it takes 2.7 us, a quarter of a small call."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device_index is None else device_index)
 
 
 class _Here:
@@ -187,6 +189,6 @@ _HERE_CTX = _Here()
 
 
 def on_device(device):
-    """Makes `device` current for a call (stream_ptr() is the current device's stream)."""
+    """Makes `device` current for a call: a kernel is launched on the device of its stream."""
     import torch
-    return _HERE_CTX if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE_CTX if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)

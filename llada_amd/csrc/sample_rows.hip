@@ -14,9 +14,9 @@
 // totals and then inside one chunk.  The row is read once and stays in registers (16 x 16 bytes a lane, 1024 lanes) for
 // the last step, which turns "the j-th entry of value v" into an index.
 //
-// The histogram has a bin for every bf16 value of magnitude in [2^-55, 2^9) of either sign and one for zero (64 KiB).  A
-// row with another finite magnitude, an infinity of positive sign or a NaN is "irregular" (its clamped bins say so, at no
-// cost to other rows) and is counted over the whole 16-bit key space in four windows instead; -inf entries, NaNs
+// The histogram has a bin for every bf16 value of magnitude in [2^-55, 2^8) of either sign and one for zero (2 x 32 KiB).
+// A row with another finite magnitude, an infinity of positive sign or a NaN is "irregular" (its clamped bins say so, at
+// no cost to other rows) and is counted over the whole 16-bit key space in four windows instead; -inf entries, NaNs
 // included, have no weight and are never drawn.  A row with nothing else gives token 0 with probability 0.
 #include "common.h"
 #include "philox.h"
@@ -27,15 +27,18 @@ namespace {
 constexpr int THREADS = ROW_THREADS;                 // 1024
 constexpr int SLOTS = ROW_SLOTS;                     // 16-byte chunks a lane
 constexpr int NWV = THREADS / 64;
-constexpr unsigned MAG_LO = 0x2400, MAG_HI = 0x4400; // magnitudes with a bin of their own: [2^-55, 2^9)
-constexpr int SPAN = MAG_HI - MAG_LO;                // 8192
-constexpr int PLANE = SPAN + 2;                      // bin 0: below the range (zero), SPAN + 1: above
-constexpr int BINS = 2 * PLANE;                      // both signs
+constexpr unsigned MAG_LO = 0x2400, MAG_HI = 0x4380; // magnitudes with a bin of their own: [2^-55, 2^8)
+constexpr int SPAN = MAG_HI - MAG_LO;                // 8064; bin 0: below the range (zero), SPAN + 1: above
+constexpr int NEGATIVE = 0x8000;                     // bin of a negative value: the sign bit stays where it is
 constexpr int REGULAR_KEYS = 2 * SPAN + 1;           // descending values: SPAN positive, zero, SPAN negative
+constexpr int REGULAR_CHUNKS = (REGULAR_KEYS + 63) / 64;
+constexpr int PER_WAVE = 16;                         // groups of 64 keys of a regular row a wave looks through
+static_assert(REGULAR_CHUNKS <= PER_WAVE * NWV && NWV == 16 && PER_WAVE == 16, "every group has a wave");
 constexpr int WINDOW = 16384;                        // irregular rows: keys counted at a time, 4 windows
 constexpr int MAX_CHUNKS = 65536 / 64;
+constexpr int REST_AT = WINDOW;                      // in LDS words: the other shared state, between the planes
+constexpr int LDS_WORDS = NEGATIVE + SPAN + 2;
 constexpr unsigned LLADA_STREAM_SAMPLE = 4u;
-static_assert(WINDOW <= BINS, "a window fits the bins");
 
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 typedef __attribute__((ext_vector_type(2))) short s16x2;
@@ -55,21 +58,21 @@ struct SampleArgs {
 };
 
 struct Shared {
-    unsigned bins[BINS];
     unsigned cnt[MAX_CHUNKS];        // entries of a chunk of 64 keys, then: entries before it
     double mass[MAX_CHUNKS];         // their weight, then: the weight before it
     double conf[NWV];                // epilogue: partial sums of the waves
-    unsigned total;
     double total_mass;
+    unsigned total;
     int first[NWV];
     int irregular;
-    // the drawn entry
-    int key, j, tied;
+    int j, tied;                     // the drawn entry: the j-th of `tied` equal ones
     float value, prob;
     unsigned slot_tot[SLOTS];
     unsigned wave_tot[NWV];
     int token;
+    unsigned short keys[REGULAR_KEYS + 64];   // regular rows: the keys that have entries, in order
 };
+static_assert(REST_AT * 4 + sizeof(Shared) <= NEGATIVE * 4 && LDS_WORDS * 4 <= 160 * 1024, "the planes leave room");
 
 // Key s of a row's value order (0 = the largest) <-> value.  Regular rows: the histogram's own order; irregular rows: all
 // bf16 patterns.
@@ -83,13 +86,11 @@ __device__ __forceinline__ float key_value(int s, bool regular) {
     return __uint_as_float(((k & 0x8000u) ? k ^ 0x8000u : ~k & 0xFFFFu) << 16);
 }
 
-__device__ __forceinline__ unsigned key_count(const Shared& sh, int s, bool regular) {
-    if (regular) {
-        if (s >= REGULAR_KEYS) return 0u;
-        if (s == SPAN) return sh.bins[0] + sh.bins[PLANE];
-        return s < SPAN ? sh.bins[SPAN - s] : sh.bins[PLANE + (s - SPAN)];
-    }
-    return sh.bins[s & (WINDOW - 1)];
+__device__ __forceinline__ unsigned key_count(const unsigned* bins, int s, bool regular) {
+    if (!regular) return bins[s & (WINDOW - 1)];
+    if (s >= REGULAR_KEYS) return 0u;
+    const unsigned n = bins[s <= SPAN ? SPAN - s : NEGATIVE + s - SPAN];
+    return s == SPAN ? n + bins[NEGATIVE] : n;
 }
 
 // irregular rows: key of a bf16 pattern, -1 for an entry without weight (-inf, NaN); -0 counts as +0
@@ -99,21 +100,33 @@ __device__ __forceinline__ int full_key(unsigned bits) {
     return 65535 - (int)((bits & 0x8000u) ? ~bits & 0xFFFFu : bits | 0x8000u);
 }
 
-__device__ __forceinline__ double wave_scan(double v, int lane) {      // inclusive, fixed order
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double t = __shfl_up(v, o);
-        if (lane >= o) v += t;
-    }
+// Scans and broadcasts by data-parallel moves: a few cycles a step where a shuffle through LDS takes a hundred.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp(unsigned v) {      // lanes without a source get 0
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t r = (uint64_t)dpp<CTRL, ROWS>((unsigned)(b >> 32)) << 32 | dpp<CTRL, ROWS>((unsigned)b);
+    return __builtin_bit_cast(double, r);
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {               // inclusive, fixed order
+    v += dpp<0x111, 0xF>(v);
+    v += dpp<0x112, 0xF>(v);
+    v += dpp<0x114, 0xF>(v);
+    v += dpp<0x118, 0xF>(v);
+    v += dpp<0x142, 0xA>(v);
+    v += dpp<0x143, 0xC>(v);
     return v;
 }
-__device__ __forceinline__ unsigned wave_scan(unsigned v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned t = __shfl_up(v, o);
-        if (lane >= o) v += t;
-    }
-    return v;
+template <class T>
+__device__ __forceinline__ T lane_before(T v) { return dpp<0x138, 0xF>(v); }      // lane 0: zero
+__device__ __forceinline__ unsigned from_lane(unsigned v, int at) { return (unsigned)__builtin_amdgcn_readlane((int)v, at); }
+__device__ __forceinline__ double from_lane(double v, int at) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)from_lane((unsigned)(b >> 32), at) << 32 | from_lane((unsigned)b, at));
 }
 __device__ __forceinline__ double wave_total(double v) {
 #pragma unroll
@@ -121,77 +134,75 @@ __device__ __forceinline__ double wave_total(double v) {
     return v;
 }
 
+// 2^y in float64, y <= 0: 2^rint(y) times the Taylor polynomial of 2^f = e^(f ln 2) to the 13th power, |f| <= 1/2
+// (remainder below 5e-18).  The argument is formed with one rounding, so a weight is off by up to 2^-53 |y| of itself:
+// what counts in a row's sums are the weights with small |y|.  Half the instructions of the library's exp, and in four
+// short chains where a wave would wait out one long one.
+__device__ __forceinline__ double exp2_neg(double y) {
+    constexpr double L = 0.69314718055994530942;
+    constexpr double C2 = L * L / 2, C3 = C2 * L / 3, C4 = C3 * L / 4, C5 = C4 * L / 5, C6 = C5 * L / 6, C7 = C6 * L / 7, C8 = C7 * L / 8,
+                     C9 = C8 * L / 9, C10 = C9 * L / 10, C11 = C10 * L / 11, C12 = C11 * L / 12, C13 = C12 * L / 13;
+    y = fmax(y, -1100.0);                        // (2^-1100 is 0; an infinity stays out of the polynomial)
+    const double k = __builtin_rint(y), f = y - k, f2 = f * f, f4 = f2 * f2;
+    const double a = __builtin_fma(__builtin_fma(C3, f, C2), f2, __builtin_fma(L, f, 1.0));
+    const double b = __builtin_fma(__builtin_fma(C7, f, C6), f2, __builtin_fma(C5, f, C4));
+    const double c = __builtin_fma(__builtin_fma(C11, f, C10), f2, __builtin_fma(C9, f, C8));
+    const double d = __builtin_fma(C13, f, C12);
+    const double p = __builtin_fma(__builtin_fma(__builtin_fma(d, f4, c), f4, b), f4, a);
+    return __builtin_ldexp(p, (int)k);
+}
+constexpr double LOG2E = 1.44269504088896340736;
+
 // (by value: a bit cast straight from a vector's element reads the vector's first)
 __device__ __forceinline__ u16x2 halves(unsigned w) { return __builtin_bit_cast(u16x2, w); }
 
-// entries v0 .. v0 + 7 of a row, -inf outside it; `vector`: v0 stands at a 16-byte boundary
-__device__ __forceinline__ u32x4 load_chunk(const bf16_t* row, int v0, int vocab, bool vector) {
-    if (vector && v0 >= 0 && v0 + 8 <= vocab) return __builtin_nontemporal_load((const u32x4*)(row + v0));
-    u32x4 t = {BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2};
+// generate.py:89-90 on eight entries
+__device__ __forceinline__ u32x4 combine(u32x4 c, u32x4 u, float cfg1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        c[e] = pack_bf16x2(cfg_combine(bf16lo(c[e]), bf16lo(u[e]), cfg1), cfg_combine(bf16hi(c[e]), bf16hi(u[e]), cfg1));
+    return c;
+}
+
+// Entries v0 .. v0 + 7 of a row as the draw sees them, one at a time: combined under guidance; -inf for what lies outside the
+// row and for the entry that is taken out of everything (EOS removed before the draw).
+template <bool EPI>
+__device__ __forceinline__ u32x4 row_chunk(const bf16_t* lc, const bf16_t* lu, int v0, int vocab, float cfg1, int excluded) {
+    u32x4 t = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int v = v0 + e;
-        if (v < 0 || v >= vocab) continue;
-        const unsigned bits = row[v];
-        t[e >> 1] = (e & 1) ? (t[e >> 1] & 0xFFFFu) | bits << 16 : (t[e >> 1] & 0xFFFF0000u) | bits;
+        unsigned bits = 0xFF80u;
+        if (v >= 0 && v < vocab && !(EPI && v == excluded)) {
+            bits = lc[v];
+            if (lu) bits = f32_to_bf16(cfg_combine(bf16_to_f32((bf16_t)bits), bf16_to_f32(lu[v]), cfg1));
+        }
+        t[e >> 1] |= bits << (16 * (e & 1));
     }
     return t;
 }
 
 // Draws the token of one row.  EPI: also leaves the row's confidence (rules of llada_remask_scores) in `conf`.
 template <bool EPI>
-__device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
+__device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
                                            double top_p, double min_p, double u, int excl_all, int excl_conf, float& conf) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int V = a.vocab;
     // The row in registers: chunk c = lane + 1024 i holds entries 8 c - off .. + 7, off = the row's offset from a 16-byte
     // boundary in entries, so that all but its first and last chunk are one aligned load.
     const int off = (int)(((uintptr_t)lc >> 1) & 7);
-    const bool uvec = lu && (int)(((uintptr_t)lu >> 1) & 7) == off;
     const int chunks = (V + off + 7) / 8;
 
-    for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0u;
+    for (int i = tid; i < (SPAN + 2 + 3) / 4; i += THREADS) {
+        ((u32x4*)bins)[i] = (u32x4){0u, 0u, 0u, 0u};
+        if (i < (SPAN + 2) / 4) ((u32x4*)(bins + NEGATIVE))[i] = (u32x4){0u, 0u, 0u, 0u};
+    }
+    if (tid < (SPAN + 2) % 4) bins[NEGATIVE + (SPAN + 2) / 4 * 4 + tid] = 0u;
     if (tid < SLOTS) sh.slot_tot[tid] = 0u;
     if (tid == 0) sh.irregular = 0;
 
-    // one chunk of the row as the draw sees it: combined under guidance; what lies outside the row, and the entry that is
-    // taken out of everything (EOS removed before the draw), as -inf
-    auto put = [](u32x4 t, int e, unsigned bits) {
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-            if (w == e) t[w >> 1] = (w & 1) ? (t[w >> 1] & 0xFFFFu) | bits << 16 : (t[w >> 1] & 0xFFFF0000u) | bits;
-        return t;
-    };
-    auto finish_chunk = [&](u32x4 t, int c) {
-        const int v0 = c * 8 - off;
-        if (lu) {
-            const u32x4 b = load_chunk(lu, v0, V, uvec);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                t[e] = pack_bf16x2(cfg_combine(bf16lo(t[e]), bf16lo(b[e]), a.cfg1), cfg_combine(bf16hi(t[e]), bf16hi(b[e]), a.cfg1));
-            if (v0 < 0 || v0 + 8 > V) {          // the combination of two -inf is a NaN
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (v0 + e < 0 || v0 + e >= V) t = put(t, e, 0xFF80u);
-            }
-        }
-        if (EPI && excl_all >= 0 && (excl_all + off) >> 3 == c) t = put(t, (excl_all + off) & 7, 0xFF80u);
-        return t;
-    };
-    const u32x4 ninf = {BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2};
-    u32x4 q[SLOTS];
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-        const int c = tid + i * THREADS;
-        q[i] = c < chunks ? load_chunk(lc, c * 8 - off, V, true) : ninf;
-    }
-    if (lu || (EPI && excl_all >= 0)) {
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-            const int c = tid + i * THREADS;
-            if (c < chunks) q[i] = finish_chunk(q[i], c);
-        }
-    }
+    __syncthreads();
+
     // an entry the confidence's softmax does not see although it can be drawn (generate.py:100-101)
     float lx_excl = -INFINITY;
     if (EPI && excl_conf >= 0) {
@@ -200,26 +211,63 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, cons
     }
     // entries of a key that this softmax sees
     auto seen = [&](unsigned n, float v) { return n - (v == lx_excl ? 1u : 0u); };
-    __syncthreads();
 
-    // ---- the histogram: clamped magnitudes, both signs ----
+    // The row in registers.  A chunk that the row covers only in part (its first or last) is fetched entry by entry, once and
+    // apart from the others: this code runs once a row, and what it costs beside its memory time is its length.
+    const u32x4 ninf = {BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2};
+    u32x4 q[SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+        const int c = tid + i * THREADS, v0 = c * 8 - off;
+        q[i] = ninf;
+        if (v0 >= 0 && v0 + 8 <= V) q[i] = __builtin_nontemporal_load((const u32x4*)(lc + v0));
+    }
+    if (lu) {
+#pragma unroll
+        for (int g = 0; g < SLOTS; g += 4) {
+            u32x4 b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int v0 = (tid + (g + i) * THREADS) * 8 - off;
+                if (v0 >= 0 && v0 + 8 <= V) b[i] = __builtin_nontemporal_load((const u32x4*)(lu + v0));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int v0 = (tid + (g + i) * THREADS) * 8 - off;
+                if (v0 >= 0 && v0 + 8 <= V) q[g + i] = combine(q[g + i], b[i], a.cfg1);
+            }
+        }
+    }
+    if (off != 0 || ((V + off) & 7) != 0 || (EPI && excl_all >= 0)) {
+        const int ex = EPI && excl_all >= 0 ? (excl_all + off) >> 3 : -1;
+#pragma unroll 1
+        for (int k = 0; k < 3; ++k) {
+            const int c = k == 0 ? 0 : k == 1 ? chunks - 1 : ex;
+            if (c < 0 || (c & (THREADS - 1)) != tid) continue;
+            const u32x4 t = row_chunk<EPI>(lc, lu, c * 8 - off, V, a.cfg1, excl_all);
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i)
+                if (i == c / THREADS) q[i] = t;
+        }
+    }
+
+    // ---- the histogram, as the chunks arrive: clamped magnitudes, both signs ----
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
         if (tid + i * THREADS >= chunks) continue;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const u16x2 w = halves(q[i][e]);
-            const u16x2 mag = w & (unsigned short)0x7FFF;
+            const u16x2 mag = halves(q[i][e] & 0x7FFF7FFFu);
             const u16x2 idx = __builtin_elementwise_min(__builtin_elementwise_sub_sat(mag, (u16x2)((unsigned short)(MAG_LO - 1))),
                                                         (u16x2)((unsigned short)(SPAN + 1)));
-            const u16x2 at = (w >> (unsigned short)15) * (unsigned short)PLANE + idx;
-            atomicAdd(&sh.bins[at[0]], 1u);
-            atomicAdd(&sh.bins[at[1]], 1u);
+            const unsigned at = __builtin_bit_cast(unsigned, idx) | (q[i][e] & 0x80008000u);
+            atomicAdd(&bins[at & 0xFFFFu], 1u);
+            atomicAdd(&bins[at >> 16], 1u);
         }
     }
     __syncthreads();
     // clamped bins that are not empty: zeros and -inf are as good as binned, anything else makes the row irregular
-    if (sh.bins[0] + sh.bins[PLANE] + sh.bins[SPAN + 1] + sh.bins[PLANE + SPAN + 1] != 0u) {
+    if (bins[0] + bins[NEGATIVE] + bins[SPAN + 1] + bins[NEGATIVE + SPAN + 1] != 0u) {
         // smallest magnitude above zero, largest positive pattern, largest negative one but -inf
         const u16x2 one = {1, 1}, minus_inf = {0xFF80, 0xFF80};
         u16x2 least = {0xFFFF, 0xFFFF}, neg = {0, 0};
@@ -239,99 +287,166 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, cons
     }
     __syncthreads();
     const bool regular = sh.irregular == 0;
-    const int n_chunks = regular ? (REGULAR_KEYS + 63) / 64 : MAX_CHUNKS;
+    const double to_log2 = LOG2E / T;            // a distance from the largest logit -> log2 of its weight
 
     // An irregular row: counts one window of its keys into the bins, from memory again (such rows are rare and the
     // row's registers are better left alone).  All threads call it together.
     auto count_window = [&](int win) {
         __syncthreads();
-        for (int i = tid; i < WINDOW; i += THREADS) sh.bins[i] = 0u;
+        for (int i = tid; i < WINDOW; i += THREADS) bins[i] = 0u;
         __syncthreads();
 #pragma unroll 1
         for (int c = tid; c < chunks; c += THREADS) {
-            const u32x4 t = finish_chunk(load_chunk(lc, c * 8 - off, V, true), c);
+            const u32x4 t = row_chunk<EPI>(lc, lu, c * 8 - off, V, a.cfg1, excl_all);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int k = full_key((e & 1) ? t[e >> 1] >> 16 : t[e >> 1] & 0xFFFFu);
-                if (k >= 0 && k / WINDOW == win) atomicAdd(&sh.bins[k & (WINDOW - 1)], 1u);
+                if (k >= 0 && k / WINDOW == win) atomicAdd(&bins[k & (WINDOW - 1)], 1u);
             }
         }
         __syncthreads();
     };
 
-    // ---- totals of the chunks: entries, weight; the largest value on the way ----
-    int top_key = 0x7fffffff;
-    float m = 0.f;
-    double s_sum = 0.0;              // epilogue: sum of exp(l - m) over the row
-    for (int win = 0; win < (regular ? 1 : 4); ++win) {
-        if (!regular) count_window(win);
-        const int c_lo = regular ? 0 : win * (WINDOW / 64), c_hi = regular ? n_chunks : c_lo + WINDOW / 64;
-        if (top_key == 0x7fffffff) {
-            int mine = 0x7fffffff;
-            for (int c = c_lo + wave; c < c_hi; c += NWV) {
-                const uint64_t any = __builtin_amdgcn_ballot_w64(key_count(sh, c * 64 + lane, regular) != 0u);
-                if (any != 0 && mine == 0x7fffffff) mine = c * 64 + __builtin_ctzll(any);
-            }
-            if (lane == 0) sh.first[wave] = mine;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < NWV; ++w) top_key = min(top_key, sh.first[w]);
-            if (top_key != 0x7fffffff) m = key_value(top_key, regular);
-            __syncthreads();
-        }
-        for (int c = c_lo + wave; c < c_hi; c += NWV) {
-            const unsigned n = key_count(sh, c * 64 + lane, regular);
-            if (__builtin_amdgcn_ballot_w64(n != 0u) == 0) {
-                if (lane == 0) {
-                    sh.cnt[c] = 0u;
-                    sh.mass[c] = 0.0;
-                }
-                continue;
-            }
-            const float v = key_value(c * 64 + lane, regular);
-            const double dl = v == m ? 0.0 : (double)v - (double)m;
-            const double wgt = T > 0.0 ? exp(dl / T) : (v == m ? 1.0 : 0.0);
-            const double ms = wave_scan(n ? n * wgt : 0.0, lane);
-            const unsigned cs = wave_scan(n, lane);
-            if (lane == 63) {
-                sh.cnt[c] = cs;
-                sh.mass[c] = ms;
-            }
-            if (EPI) s_sum += n ? seen(n, v) * exp(dl) : 0.0;
-        }
-    }
-    __syncthreads();
-
-    // key s: its value minus the largest, its weight
-    auto distance = [&](int s) {
-        const float v = key_value(s, regular);
+    // The row's values in order stand at positions 0 .. n_pos - 1: a regular row's occupied keys, gathered in a list; an
+    // irregular row's whole key space.  A chunk is 64 positions.
+    float m = 0.f;                   // the largest value
+    int n_pos = 65536;
+    auto key_at = [&](int p) { return regular ? (int)sh.keys[p] : p; };
+    // position p: its value minus the largest, the weight at that distance
+    auto distance = [&](int p) {
+        const float v = key_value(key_at(p), regular);
         return v == m ? 0.0 : (double)v - (double)m;
     };
-    auto weight = [&](int s) {
-        const double dl = distance(s);
-        return T > 0.0 ? exp(dl / T) : (dl == 0.0 ? 1.0 : 0.0);
+    auto weight_at = [&](double dl) { return dl == 0.0 ? 1.0 : T > 0.0 ? exp2_neg(dl * to_log2) : 0.0; };
+    double s_sum = 0.0;              // epilogue: sum of exp(l - m) over the row
+    auto total_chunk = [&](int c) {
+        const int p = c * 64 + lane;
+        unsigned n = 0;
+        double dl = 0.0;
+        if (p < n_pos) {
+            const int s = key_at(p);
+            n = key_count(bins, s, regular);
+            const float v = key_value(s, regular);
+            dl = v == m ? 0.0 : (double)v - (double)m;
+            if (EPI && n) s_sum += seen(n, v) * exp2_neg(dl * LOG2E);
+        }
+        const double ms = wave_scan(n ? n * weight_at(dl) : 0.0);
+        const unsigned cs = wave_scan(n);
+        if (lane == 63) {
+            sh.cnt[c] = cs;
+            sh.mass[c] = ms;
+        }
     };
 
-    // ---- exclusive prefixes over the chunks (one wave, 64 chunks at a time) ----
-    if (wave == 0) {
-        unsigned cb = 0;
-        double qb = 0.0;
-#pragma unroll 1
-        for (int at = lane; at < (n_chunks + 63) / 64 * 64; at += 64) {
-            const unsigned c = at < n_chunks ? sh.cnt[at] : 0u;
-            const double w = at < n_chunks ? sh.mass[at] : 0.0;
-            const unsigned ci = wave_scan(c, lane);
-            const double wi = wave_scan(w, lane);
-            double we = __shfl_up(wi, 1);
-            if (lane == 0) we = 0.0;
-            sh.cnt[at] = cb + ci - c;
-            sh.mass[at] = qb + we;
-            cb += __shfl(ci, 63);
-            qb += __shfl(wi, 63);
+    // ---- totals of the chunks: entries, weight ----
+    if (regular) {
+        // group i * 16 + wave of 64 keys: neighbouring groups, which are full together, are spread over the waves
+        unsigned n[PER_WAVE];
+#pragma unroll
+        for (int i = 0; i < PER_WAVE; ++i) {
+            const int s = (i * NWV + wave) * 64 + lane;
+            n[i] = bins[s <= SPAN ? SPAN - s : NEGATIVE + min(s - SPAN, SPAN + 1)];
+            if (i == SPAN / 64 / NWV && s == SPAN) n[i] += bins[NEGATIVE];          // zero of either sign
+            if (i == PER_WAVE - 1 && s >= REGULAR_KEYS) n[i] = 0u;
         }
-        if (lane == 0) {
-            sh.total = cb;
-            sh.total_mass = qb;
+        uint64_t any[PER_WAVE];
+        unsigned held = 0;
+#pragma unroll
+        for (int i = 0; i < PER_WAVE; ++i) {
+            any[i] = __builtin_amdgcn_ballot_w64(n[i] != 0u);
+            if (lane == i) held = (unsigned)__popcll(any[i]);
+        }
+        if (lane < PER_WAVE) sh.cnt[lane * NWV + wave] = held;
+        __syncthreads();
+        // where each group's keys go in the list: a scan over the 256 groups, in every wave
+        const u32x4 g = *(const u32x4*)&sh.cnt[lane * 4];
+        const unsigned upto = wave_scan(g[0] + g[1] + g[2] + g[3]);
+        n_pos = (int)from_lane(upto, 63);
+        unsigned base = upto - (g[0] + g[1] + g[2] + g[3]);
+        const int j = wave & 3;
+        base += (j > 0 ? g[0] : 0u) + (j > 1 ? g[1] : 0u) + (j > 2 ? g[2] : 0u);
+#pragma unroll
+        for (int i = 0; i < PER_WAVE; ++i) {
+            const unsigned before = __builtin_amdgcn_mbcnt_hi((unsigned)(any[i] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)any[i], 0u));
+            if (n[i]) sh.keys[from_lane(base, 4 * i + (wave >> 2)) + before] = (unsigned short)((i * NWV + wave) * 64 + lane);
+        }
+        __syncthreads();
+        if (n_pos > 0) m = key_value(sh.keys[0], true);
+#pragma unroll 1
+        for (int c = wave; c * 64 < n_pos; c += NWV) total_chunk(c);
+    } else {
+        bool found = false;
+        for (int win = 0; win < 4; ++win) {
+            count_window(win);
+            const int c_lo = win * (WINDOW / 64), c_hi = c_lo + WINDOW / 64;
+            if (!found) {
+                int mine = 0x7fffffff;
+                for (int c = c_lo + wave; c < c_hi; c += NWV) {
+                    const uint64_t any = __builtin_amdgcn_ballot_w64(key_count(bins, c * 64 + lane, false) != 0u);
+                    if (any != 0 && mine == 0x7fffffff) mine = c * 64 + __builtin_ctzll(any);
+                }
+                if (lane == 0) sh.first[wave] = mine;
+                __syncthreads();
+                int top = 0x7fffffff;
+#pragma unroll
+                for (int w = 0; w < NWV; ++w) top = min(top, sh.first[w]);
+                found = top != 0x7fffffff;
+                if (found) m = key_value(top, false);
+                __syncthreads();
+            }
+            for (int c = c_lo + wave; c < c_hi; c += NWV) total_chunk(c);
+        }
+    }
+    const int n_chunks = (n_pos + 63) / 64;
+    __syncthreads();
+
+    // ---- exclusive prefixes over the chunks (wave 0); a regular row's stay in its registers: chunks 4 lane .. + 3 ----
+    unsigned pc[4] = {0u, 0u, 0u, 0u};
+    double pm[4] = {0.0, 0.0, 0.0, 0.0};
+    if (wave == 0) {
+        if (regular) {
+            unsigned c[4];
+            double w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool there = lane * 4 + i < n_chunks;
+                c[i] = there ? sh.cnt[lane * 4 + i] : 0u;
+                w[i] = there ? sh.mass[lane * 4 + i] : 0.0;
+            }
+            const unsigned ci = wave_scan(c[0] + c[1] + c[2] + c[3]);
+            const double wi = wave_scan(w[0] + w[1] + w[2] + w[3]);
+            pc[0] = lane_before(ci);
+            pm[0] = lane_before(wi);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                pc[i] = pc[i - 1] + c[i - 1];
+                pm[i] = pm[i - 1] + w[i - 1];
+            }
+            *(u32x4*)&sh.cnt[lane * 4] = (u32x4){pc[0], pc[1], pc[2], pc[3]};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sh.mass[lane * 4 + i] = pm[i];
+            if (lane == 63) {
+                sh.total = ci;
+                sh.total_mass = wi;
+            }
+        } else {
+            unsigned cb = 0;
+            double qb = 0.0;
+#pragma unroll 1
+            for (int at = lane; at < MAX_CHUNKS; at += 64) {
+                const unsigned c = sh.cnt[at];
+                const double w = sh.mass[at];
+                const unsigned ci = wave_scan(c);
+                const double wi = wave_scan(w);
+                sh.cnt[at] = cb + ci - c;
+                sh.mass[at] = qb + lane_before(wi);
+                cb += from_lane(ci, 63);
+                qb += from_lane(wi, 63);
+            }
+            if (lane == 0) {
+                sh.total = cb;
+                sh.total_mass = qb;
+            }
         }
     }
     __syncthreads();
@@ -346,24 +461,18 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, cons
         return;
     }
 
-    // An irregular row's bins hold one window: count the one that holds chunk c again (uniform over the workgroup).
-    // A regular row's searches run in wave 0 alone, an irregular row's with every wave following.
-    auto chunk_of_count = [&](unsigned k) {          // chunk that holds the k-th entry (k >= 1)
+    // A regular row's searches run in wave 0 alone.  An irregular row's bins hold one window at a time: every wave follows
+    // the search, and the window that holds a chunk is counted again when it is looked into.
+    auto chunks_before = [&](auto&& test) {          // number of leading chunks whose prefixes pass the test
         int c = 0;
+        if (regular) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c += __popcll(__builtin_amdgcn_ballot_w64(lane * 4 + i < n_chunks && test(pc[i], pm[i])));
+        } else {
 #pragma unroll 1
-        for (int at = lane; at < (n_chunks + 63) / 64 * 64; at += 64) {
-            c += __popcll(__builtin_amdgcn_ballot_w64(at < n_chunks && sh.cnt[at] < k));
+            for (int at = lane; at < MAX_CHUNKS; at += 64) c += __popcll(__builtin_amdgcn_ballot_w64(test(sh.cnt[at], sh.mass[at])));
         }
-        return c - 1;
-    };
-    auto chunk_of_mass = [&](double x, bool strict) {  // last chunk whose prefix is below x (strict: at most x)
-        int c = 0;
-#pragma unroll 1
-        for (int at = lane; at < (n_chunks + 63) / 64 * 64; at += 64) {
-            const bool before = at < n_chunks && (strict ? sh.mass[at] <= x : sh.mass[at] < x);
-            c += __popcll(__builtin_amdgcn_ballot_w64(before));
-        }
-        return c > 0 ? c - 1 : 0;
+        return c;
     };
     struct Inside {          // a chunk, entry by entry of its keys
         unsigned n, upto;    // this lane's key: entries, entries of the row up to and with it
@@ -372,51 +481,54 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, cons
     auto look_inside = [&](int c) {
         if (!regular) count_window(c / (WINDOW / 64));
         Inside x;
-        x.n = key_count(sh, c * 64 + lane, regular);
-        x.w = x.n ? weight(c * 64 + lane) : 0.0;
-        const double own = x.n ? x.n * x.w : 0.0;
-        const double incl = wave_scan(own, lane);
-        double ex = __shfl_up(incl, 1);
-        if (lane == 0) ex = 0.0;
-        x.before = sh.mass[c] + ex;
-        x.upto = sh.cnt[c] + wave_scan(x.n, lane);
+        const int p = c * 64 + lane;
+        x.n = p < n_pos ? key_count(bins, key_at(p), regular) : 0u;
+        x.w = x.n ? weight_at(distance(p)) : 0.0;
+        x.before = sh.mass[c] + lane_before(wave_scan(x.n ? x.n * x.w : 0.0));
+        x.upto = sh.cnt[c] + wave_scan(x.n);
         return x;
     };
-    // weight of the first k entries of the row (1 <= k <= N)
-    auto mass_of = [&](unsigned k) {
-        if (k >= N) return sh.total_mass;
-        const Inside x = look_inside(chunk_of_count(k));
-        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(x.upto >= k && x.n != 0u));
-        return __shfl(x.before + (double)(k - (x.upto - x.n)) * x.w, at);
+    auto chunk_of_rank = [&](unsigned k) {           // chunk that holds the k-th entry (k >= 1)
+        return chunks_before([&](unsigned c, double) { return c < k; }) - 1;
     };
 
     if (wave == 0 || !regular) {
         unsigned kept = top_k > 0 && (unsigned)top_k < N ? (unsigned)top_k : N;
+        double total = sh.total_mass;                              // weight of the first `kept` entries
         if (!(T > 0.0)) kept = 1u;                                 // the largest logit, lowest index
+        if (kept == 1u) {
+            total = 1.0;
+        } else if (kept < N) {
+            const Inside x = look_inside(chunk_of_rank(kept));
+            const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(x.upto >= kept && x.n != 0u));
+            total = from_lane(x.before + (double)(kept - (x.upto - x.n)) * x.w, at);
+        }
         if (top_p < 1.0 && kept > 1u) {
-            const double x = top_p * mass_of(kept);
-            int c = chunk_of_mass(x, false);
-            const Inside y = look_inside(c);
+            const double x = top_p * total;
+            const Inside y = look_inside(max(chunks_before([&](unsigned, double w) { return w < x; }) - 1, 0));
             // the first key of the chunk whose own entries reach x (none: x is a rounding short of the next chunk)
             const uint64_t reach = __builtin_amdgcn_ballot_w64(y.n != 0u && y.before + y.n * y.w >= x);
             if (reach != 0) {
                 const int at = __builtin_ctzll(reach);
-                const double w = __shfl(y.w, at), before = __shfl(y.before, at);
-                const unsigned n = __shfl(y.n, at), upto = __shfl(y.upto, at);
+                const double w = from_lane(y.w, at), before = from_lane(y.before, at);
+                const unsigned n = from_lane(y.n, at), upto = from_lane(y.upto, at);
                 unsigned j = w > 0.0 ? (unsigned)fmin(fmax(ceil((x - before) / w), 1.0), (double)n) : 1u;
                 while (j > 1u && before + (double)(j - 1u) * w >= x) --j;
                 while (j < n && before + (double)j * w < x) ++j;
-                kept = min(kept, upto - n + j);
-            } else {
-                kept = max(min(kept, __shfl(y.upto, 63)), 1u);
+                if (upto - n + j < kept) {
+                    kept = upto - n + j;
+                    total = before + (double)j * w;
+                }
+            } else if (from_lane(y.upto, 63) < kept) {
+                kept = max(from_lane(y.upto, 63), 1u);
+                total = from_lane(y.before + y.n * y.w, 63);
             }
         }
         if (min_p > 0.0 && kept > 1u) {
-            // the first key whose weight is below min_p: weights fall with the key, 64 probes a round.  Compared before the
+            // the first position whose weight is below min_p: weights fall along the positions, 64 probes a round.  Compared before the
             // exponential: min_p = 1 keeps exactly the entries that equal the largest, whatever T.
             const double edge = T * log(min_p);
-            int cut = 0, hi = regular ? REGULAR_KEYS : 65536;
-            const int keys = hi;
+            int cut = 0, hi = n_pos;
             while (cut < hi) {
                 const int step = (hi - cut + 63) / 64, s = cut + (lane + 1) * step - 1;
                 const uint64_t fails = __builtin_amdgcn_ballot_w64(s >= hi || distance(s) < edge);
@@ -424,99 +536,117 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, cons
                 hi = min(hi, cut + (f + 1) * step - 1);
                 cut = cut + f * step;
             }
-            unsigned nm = N;
-            if (cut < keys) {
-                const int c = cut / 64;
-                const Inside x = look_inside(c);
-                nm = __shfl(x.upto - x.n, cut & 63);
+            if (cut < n_pos) {
+                const Inside x = look_inside(cut / 64);
+                const unsigned nm = from_lane(x.upto - x.n, cut & 63);
+                if (nm < kept) {
+                    kept = max(nm, 1u);
+                    total = nm > 0u ? from_lane(x.before, cut & 63) : 1.0;
+                }
             }
-            kept = min(kept, nm > 0u ? nm : 1u);
         }
-        const double total = mass_of(kept);
         const double x = u * total;
-        const int c = chunk_of_mass(x, true);
-        const Inside y = look_inside(c);
+        int c = max(chunks_before([&](unsigned, double w) { return w <= x; }) - 1, 0);
+        Inside y = look_inside(c);
         const uint64_t over = __builtin_amdgcn_ballot_w64(y.n != 0u && y.before + y.n * y.w > x);
-        unsigned rank = min(kept, __shfl(y.upto, 63) + 1u);        // 1-based; as it stands: x rounds up to the chunk's end
+        int at = 0;
+        unsigned rank = from_lane(y.upto, 63) + 1u;                // 1-based; as it stands: x rounds up to the chunk's end
         if (over != 0) {
-            const int at = __builtin_ctzll(over);
-            const double w = __shfl(y.w, at), before = __shfl(y.before, at);
-            const unsigned n = __shfl(y.n, at), upto = __shfl(y.upto, at);
+            at = __builtin_ctzll(over);
+            const double w = from_lane(y.w, at), before = from_lane(y.before, at);
+            const unsigned n = from_lane(y.n, at), upto = from_lane(y.upto, at);
             unsigned j = w > 0.0 ? (unsigned)fmin(fmax((x - before) / w, 0.0), (double)(n - 1u)) : 0u;
             while (j > 0u && before + (double)j * w > x) --j;
             while (j + 1u < n && before + (double)(j + 1u) * w <= x) ++j;
-            rank = min(kept, upto - n + j + 1u);
+            rank = upto - n + j + 1u;
         }
-        // the key and place of that rank
-        const Inside z = look_inside(chunk_of_count(rank));
-        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(z.n != 0u && z.upto >= rank));
-        const int cz = chunk_of_count(rank);
+        if (over == 0 || rank > kept) {                            // (a rounding past the last kept entry)
+            rank = min(rank, kept);
+            c = chunk_of_rank(rank);
+            y = look_inside(c);
+            at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(y.n != 0u && y.upto >= rank));
+        }
         if (wave == 0 && lane == at) {
-            sh.key = cz * 64 + lane;
-            sh.j = (int)(rank - (z.upto - z.n) - 1u);
-            sh.tied = (int)z.n;
-            sh.value = key_value(cz * 64 + lane, regular);
-            sh.prob = (float)(z.w / total);
+            sh.j = (int)(rank - (y.upto - y.n) - 1u);
+            sh.tied = (int)y.n;
+            sh.value = key_value(key_at(c * 64 + lane), regular);
+            sh.prob = (float)(y.w / total);
         }
     }
     __syncthreads();
 
     // ---- the j-th entry of that value, in index order ----
     const float value = sh.value;
-    unsigned mine[SLOTS / 4];                    // matches of each chunk, a byte each
+    const unsigned bits = __float_as_uint(value) >> 16;
+    const unsigned pat = bits * 0x00010001u;
+    const unsigned msk = bits == 0u ? 0x7FFF7FFFu : 0xFFFFFFFFu;      // zero: either sign
+    const bool single = sh.tied == 1;            // (uniform)
+    unsigned hits = 0;                           // chunks of this lane with a match
+    auto nearest = [&](int i) {                  // zero in a half: a match in that half of some word of chunk i
+        u16x2 x[4];
 #pragma unroll
-    for (int i = 0; i < SLOTS / 4; ++i) mine[i] = 0u;
-    {
-        const unsigned bits = __float_as_uint(value) >> 16;
-        const unsigned pat = bits * 0x00010001u, msk = bits == 0u ? 0x7FFF7FFFu : 0xFFFFFFFFu;    // zero: either sign
+        for (int e = 0; e < 4; ++e) x[e] = halves((q[i][e] ^ pat) & msk);
+        return __builtin_elementwise_min(__builtin_elementwise_min(x[0], x[1]), __builtin_elementwise_min(x[2], x[3]));
+    };
+    auto zero_half = [](u16x2 v) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        return ((b & 0xFFFFu) == 0u) | (b < 0x10000u);
+    };
+#pragma unroll
+    for (int g = 0; g < SLOTS; g += 4) {         // most waves hold no match: four chunks are ruled out at a time
+        u16x2 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = nearest(g + i);
+        if (__builtin_amdgcn_ballot_w64(zero_half(__builtin_elementwise_min(__builtin_elementwise_min(x[0], x[1]), __builtin_elementwise_min(x[2], x[3])))) == 0) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hits |= (unsigned)zero_half(x[i]) << (g + i);
+    }
+    int slot = single && hits ? __builtin_ctz(hits) : -1;     // the chunk that holds the entry, in the lane that holds it
+    unsigned skip = 0;                                        // matches of that chunk before the entry
+    if (!single) {
+        unsigned mine[SLOTS / 4] = {};           // matches of each chunk, a byte each
+        const u16x2 one = {1, 1};
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) {
+            if (__builtin_amdgcn_ballot_w64((hits >> i) & 1u) == 0) continue;
             u16x2 miss = {0, 0};
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                miss += __builtin_elementwise_min(halves((q[i][e] ^ pat) & msk), (u16x2)((unsigned short)1));
-            mine[i >> 2] |= (8u - (unsigned)(miss[0] + miss[1])) << (8 * (i & 3));
+            for (int e = 0; e < 4; ++e) miss += __builtin_elementwise_min(halves((q[i][e] ^ pat) & msk), one);
+            const unsigned n = 8u - (unsigned)(miss[0] + miss[1]);
+            mine[i >> 2] |= n << (8 * (i & 3));
+            const unsigned sum = wave_scan(n);
+            if (lane == 63) atomicAdd(&sh.slot_tot[i], sum);
+        }
+        __syncthreads();
+        const unsigned upto = wave_scan(lane < SLOTS ? sh.slot_tot[lane & (SLOTS - 1)] : 0u);
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > (unsigned)sh.j));
+        const unsigned left = (unsigned)sh.j - from_lane(lane_before(upto), at);
+        unsigned n_here = 0;
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i)
+            if (i == at) n_here = (mine[i >> 2] >> (8 * (i & 3))) & 255u;
+        const unsigned incl = wave_scan(n_here);
+        if (lane == 63) sh.wave_tot[wave] = incl;
+        __syncthreads();
+        const unsigned waves = wave_scan(lane < NWV ? sh.wave_tot[lane & (NWV - 1)] : 0u);
+        const unsigned before = from_lane(lane_before(waves), wave) + incl - n_here;
+        if (left >= before && left < before + n_here) {
+            slot = at;
+            skip = left - before;
         }
     }
-    if ((mine[0] | mine[1] | mine[2] | mine[3]) != 0u) {
+    if (slot >= 0) {
+        u32x4 t = q[0];
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-            const unsigned n = (mine[i >> 2] >> (8 * (i & 3))) & 255u;
-            if (n) atomicAdd(&sh.slot_tot[i], n);
-        }
-    }
-    __syncthreads();
-    unsigned left = (unsigned)sh.j;
-    int slot = 0;
-#pragma unroll 1
-    while (slot < SLOTS - 1 && left >= sh.slot_tot[slot]) left -= sh.slot_tot[slot++];
-    unsigned n_here = 0;
-    u32x4 here = ninf;
+        for (int i = 1; i < SLOTS; ++i)
+            if (i == slot) t = q[i];
+        unsigned ahead = 0;
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i)
-        if (i == slot) {
-            n_here = (mine[i >> 2] >> (8 * (i & 3))) & 255u;
-            here = q[i];
+        for (int e = 0; e < 8; ++e) {
+            const bool match = ((e & 1) ? bf16hi(t[e >> 1]) : bf16lo(t[e >> 1])) == value;
+            if (match && ahead == skip) sh.token = (tid + slot * THREADS) * 8 - off + e;
+            ahead += match;
         }
-    const unsigned incl = wave_scan(n_here, lane);
-    if (lane == 63) sh.wave_tot[wave] = incl;
-    __syncthreads();
-    unsigned before = incl - n_here;
-#pragma unroll 1
-    for (int w = 0; w < wave; ++w) before += sh.wave_tot[w];
-    if (left >= before && left < before + n_here) {
-        unsigned skip = left - before;
-        int found = 0;
-#pragma unroll
-        for (int e = 7; e >= 0; --e) {
-            // entries are scanned downwards: the (n_here - 1 - skip)-th match from the end
-            const float v = (e & 1) ? bf16hi(here[e >> 1]) : bf16lo(here[e >> 1]);
-            if (v == value) {
-                if (n_here - 1u == skip) found = e;
-                --n_here;
-            }
-        }
-        sh.token = (tid + slot * THREADS) * 8 - off + found;
     }
     __syncthreads();
 
@@ -546,11 +676,13 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, cons
             };
             for (int win = 0; win < (regular ? 1 : 4); ++win) {
                 if (!regular) count_window(win);
-                const int c_lo = regular ? 0 : win * (WINDOW / 64), c_hi = regular ? n_chunks : c_lo + WINDOW / 64;
-                for (int c = c_lo + wave; c < c_hi; c += NWV) {
-                    const unsigned n = key_count(sh, c * 64 + lane, regular);
+                const int p_lo = regular ? 0 : win * WINDOW, p_hi = regular ? n_pos : p_lo + WINDOW;
+#pragma unroll 1
+                for (int p = p_lo + tid; p < p_hi; p += THREADS) {
+                    const int s = key_at(p);
+                    const unsigned n = key_count(bins, s, regular);
                     if (n == 0u) continue;
-                    const float v = key_value(c * 64 + lane, regular);
+                    const float v = key_value(s, regular);
                     es += seen(n, v) * term(v == m ? 0.0 : (double)v - (double)m);
                 }
             }
@@ -570,7 +702,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared& sh, cons
 // One workgroup per row.
 template <bool EPI>
 __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const SampleArgs a) {
-    __shared__ Shared sh;
+    __shared__ __attribute__((aligned(16))) unsigned lds[LDS_WORDS];
+    Shared& sh = *(Shared*)(lds + REST_AT);
     const int row = blockIdx.x;
     const int tid = threadIdx.x;
     int pos = row, b = row, col = 0;
@@ -598,7 +731,7 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const SampleArgs a
     const int ex_all = EPI && (a.r.flags & LLADA_FLAG_LOGITS_EOS_INF) ? a.r.eos_id : -1;
     const int ex_conf = EPI && (a.r.flags & LLADA_FLAG_CONF_EOS_EOT_INF) && a.r.eot_id != ex_all ? a.r.eot_id : -1;
     float conf = 0.f;
-    sample_row<EPI>(a, sh, lc, lu, T, top_k, top_p, min_p, u, ex_all, ex_conf, conf);
+    sample_row<EPI>(a, lds, sh, lc, lu, T, top_k, top_p, min_p, u, ex_all, ex_conf, conf);
     if (tid != 0) return;
     if constexpr (EPI) {
         if (a.r.remasking == LLADA_REMASK_RANDOM) {
@@ -645,6 +778,8 @@ extern "C" int llada_sample_rows(const void* logits, const void* uncond_logits, 
     LLADA_CHECK_ARG(logits && tokens && n_rows > 0 && vocab > 0, "sample_rows: bad argument");
     LLADA_CHECK_ARG(row_stride >= vocab || n_rows == 1, "sample_rows: rows overlap (stride %lld, vocab %d)", (long long)row_stride, vocab);
     LLADA_CHECK_ARG((((uintptr_t)logits | (uintptr_t)uncond_logits) & 1) == 0, "sample_rows: misaligned logits");
+    LLADA_CHECK_ARG(uncond_logits == nullptr || (((uintptr_t)logits ^ (uintptr_t)uncond_logits) & 15) == 0,
+                    "sample_rows: uncond_logits must stand at the same offset from a 16-byte boundary as logits");
     const bool aligned = ((uintptr_t)logits & 15) == 0 && (row_stride % 8 == 0 || n_rows == 1);
     LLADA_CHECK_SUPPORTED(vocab <= ROW_MAX_VOCAB - (aligned ? 0 : 7), "sample_rows: vocab=%d: a row must fit the registers of a workgroup", vocab);
     const int rc = check_sampling("sample_rows", sampling);

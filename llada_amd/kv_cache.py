@@ -30,6 +30,7 @@ class KVCache8:
         self.layer_bytes = self.lib.llada_kv8_layer_bytes(n_seq, seq_len, n_heads)
         self.data = torch.zeros((n_layers, self.layer_bytes), dtype=torch.uint8, device=device)
         self.device = self.data.device
+        self._index = self.device.index
         n_tiles = n_seq * n_heads * ((seq_len + 63) // 64)
         self.data[:, :n_tiles * 8].view(torch.float32).fill_(1.0)      # the scales of all-zero blocks
         self._base = self.data.data_ptr()
@@ -46,14 +47,17 @@ class KVCache8:
 
     def _rows(self, x, n, width, what):
         """x as n rows a sequence at one row stride: (tensor kept alive, row stride)."""
+        shape, st = x.shape, x.stride()
         if x.dtype != torch.bfloat16 or x.device != self.device:
             raise ValueError(f"{what}: bfloat16 on {self.device} is wanted, not {x.dtype} on {x.device}")
-        shape = tuple(x.shape)
-        if len(shape) not in (2, 3) or shape[-1] < width or (shape[:-1] != (self.n_seq, n) and shape[:-1] != (self.n_seq * n,)):
+        if len(shape) == 3:
+            ok, row = shape[0] == self.n_seq and shape[1] == n, st[1] if n > 1 else st[0]
+            even = self.n_seq == 1 or st[0] == n * row
+        else:
+            ok, row, even = len(shape) == 2 and shape[0] == self.n_seq * n, st[0], True
+        if not ok or shape[-1] < width:
             raise ValueError(f"{what}: [{self.n_seq}, {n}, >= {width}] is wanted, not {list(shape)}")
-        st = x.stride()
-        row = st[-2] if n > 1 or len(shape) == 2 else st[0]
-        if st[-1] != 1 or row < width or row % 8 or x.data_ptr() % 16 or (len(shape) == 3 and shape[0] > 1 and st[0] != n * row):
+        if st[-1] != 1 or row < width or row % 8 or not even or x.data_ptr() % 16:
             x = x[..., :width].clone(memory_format=torch.contiguous_format)
             row = width
         return x, row
@@ -93,7 +97,7 @@ class KVCache8:
         m = self._mask(key_mask)
         with self._on_device():
             _lib.check(self.lib.llada_kv8_write(x.data_ptr(), stride, _lib.ptr(m), at, self._type, self.n_seq, self.seq_len,
-                                                self.n_heads, start, length, _lib.stream_ptr()))
+                                                self.n_heads, start, length, _lib.stream_ptr(self._index)))
 
     def read(self, layer):
         """The values ``layer`` stands for: (keys, values), bf16 [n_seq, seq_len, n_heads, 128]."""
@@ -102,7 +106,7 @@ class KVCache8:
             out = torch.empty((2, self.n_seq, self.seq_len, self.n_heads, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
             k, v = out[0], out[1]
             _lib.check(self.lib.llada_kv8_read(at, self._type, k.data_ptr(), v.data_ptr(), self.n_seq, self.seq_len,
-                                               self.n_heads, _lib.stream_ptr()))
+                                               self.n_heads, _lib.stream_ptr(self._index)))
         return k, v
 
     def attend(self, layer, q, key_mask=None, block=None, block_start=0, out=None):
@@ -136,5 +140,5 @@ class KVCache8:
             ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
             _lib.check(self.lib.llada_attn_kv8(qx.data_ptr(), q_stride, n_q, at, self._type, _lib.ptr(m), out.data_ptr(), self.n_seq,
                                                self.seq_len, self.n_heads, _lib.ptr(bx), b_stride, block_start, b_len,
-                                               _lib.ptr(ws), need, _lib.stream_ptr()))
+                                               _lib.ptr(ws), need, _lib.stream_ptr(self._index)))
         return out

@@ -47,30 +47,27 @@ def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uni
         if uncond_logits.shape != logits.shape or uncond_logits.dtype != torch.bfloat16 or uncond_logits.device != dev:
             raise ValueError("uncond_logits: the shape, type and device of logits are wanted")
         un = uncond_logits.reshape(-1, vocab)
-        if un.stride() != rows.stride():
-            rows, un, stride = rows.contiguous(), un.contiguous(), vocab
-    keep = []
-
-    def per_row(v, dtype):
-        if not isinstance(v, torch.Tensor):
-            return None
-        if v.dim() and v.shape != lead:
-            raise ValueError(f"a sampling parameter has shape {list(v.shape)}, the rows {list(lead)}")
-        keep.append(v.to(device=dev, dtype=dtype).expand(lead).reshape(-1).contiguous())
-        return keep[-1].data_ptr()
-
-    arrays = [per_row(temperature, torch.float32), per_row(top_k, torch.int32), per_row(top_p, torch.float32), per_row(min_p, torch.float32)]
-    t, k, p, q = (d if a is not None else v for v, d, a in zip((temperature, top_k, top_p, min_p), (1.0, 0, 1.0, 0.0), arrays))
+        if un.stride() != rows.stride() or (un.data_ptr() - rows.data_ptr()) % 16:
+            rows, un, stride = rows.clone(memory_format=torch.contiguous_format), un.clone(memory_format=torch.contiguous_format), vocab
+    arrays, keep = [None] * 4, []
+    scalars = [temperature, top_k, top_p, min_p]
+    for i, (v, dtype, off) in enumerate(zip(scalars, (torch.float32, torch.int32, torch.float32, torch.float32), (1.0, 0, 1.0, 0.0))):
+        if isinstance(v, torch.Tensor):
+            if v.dim() and v.shape != lead:
+                raise ValueError(f"a sampling parameter has shape {list(v.shape)}, the rows {list(lead)}")
+            keep.append(v.to(device=dev, dtype=dtype).expand(lead).reshape(-1).contiguous())
+            arrays[i], scalars[i] = keep[-1].data_ptr(), off
+    t, k, p, q = scalars
     u = None
     if uniforms is not None:
         if uniforms.shape != lead or uniforms.device != dev:
             raise ValueError(f"uniforms: shape {list(lead)} on {dev} is wanted")
-        u = uniforms.to(torch.float64).reshape(-1).contiguous()
+        u = uniforms if uniforms.dtype == torch.float64 and uniforms.is_contiguous() else uniforms.to(torch.float64).contiguous()
     with _lib.on_device(dev):
         tokens = torch.empty(lead, dtype=torch.int64, device=dev)
         probs = torch.empty(lead, dtype=torch.float32, device=dev) if return_probs else None
         if n:
             s = _lib.Sampling(float(t), float(p), float(q), int(k), *arrays, _lib.ptr(u))
             _lib.check(lib.llada_sample_rows(rows.data_ptr(), _lib.ptr(un), stride, float(cfg_scale), n, vocab, C.byref(s), seed, step,
-                                             row_offset, tokens.data_ptr(), _lib.ptr(probs), _lib.stream_ptr()))
+                                             row_offset, tokens.data_ptr(), _lib.ptr(probs), _lib.stream_ptr(dev.index)))
     return (tokens, probs) if return_probs else tokens

@@ -35,7 +35,7 @@ def call(lib, sampling=True, **k):
 @pytest.mark.parametrize("bad", [dict(logits=None), dict(tokens=None), dict(n=0), dict(V=0), dict(stride=63), dict(temperature=-0.1),
                                  dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_k=-1), dict(top_p=0.0),
                                  dict(top_p=1.01), dict(top_p=float("nan")), dict(min_p=-0.1), dict(min_p=1.5), dict(min_p=float("nan")),
-                                 dict(sampling=False), dict(logits=C.c_void_p(257))])
+                                 dict(sampling=False), dict(logits=C.c_void_p(257)), dict(un=C.c_void_p(258))])
 def test_refusals(lib, bad):
     from llada_amd import _lib
     assert call(lib, **bad) == _lib.ERR_INVALID and lib.llada_last_error()
