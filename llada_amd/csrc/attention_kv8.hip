@@ -24,12 +24,13 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+typedef __attribute__((address_space(3))) void* lds_void_ptr;
+typedef const __attribute__((address_space(1))) void* gbl_void_ptr;
 
 constexpr int QW = 32;                       // queries of a wave
-constexpr int NWAVES = 4;
+constexpr int NW = 4;                        // waves of a workgroup
 constexpr int OROW = KV8_HD * 4 + 16;        // bytes of a float32 output row in LDS (16 bytes of padding)
-constexpr int SLICE = QW * OROW;             // one wave's LDS: a 64 x 256-byte tile of fresh values, or its result
-static_assert(SLICE >= KV8_TOKENS * 256, "a wave's slice holds a tile of fresh values");
+constexpr int SLICE = QW * OROW;             // one wave's result in LDS
 
 template <int TYPE>
 __device__ __forceinline__ bf16x8 codes_to_bf16(unsigned a, unsigned b) {
@@ -41,6 +42,9 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(unsigned a, unsigned b) {
         const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
         r = (bf16x8){x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
     } else {
+        // (opaque to the optimiser, which would otherwise carry a prefetched tile around the loop as 256 converted
+        // floats instead of 32 words of codes, in scratch memory)
+        asm("" : "+v"(a), "+v"(b));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             r[i] = (__bf16)(float)(signed char)(a >> (8 * i));
@@ -124,10 +128,10 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[2], uint64_t valid, flo
 // tiles among themselves, their results merged once at the end; many -> each wave has queries of its own and the waves
 // meet a tile's codes in the CU's cache.
 template <int TYPE, int NQ>
-__global__ void __launch_bounds__(NWAVES * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
-    constexpr int NK = NWAVES / NQ;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[NWAVES * SLICE + NWAVES * QW * 8];
-    float* const ml = (float*)(lds + NWAVES * SLICE);       // [wave][query][2]
+__global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
+    constexpr int NK = NW / NQ;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[NW * SLICE + NW * QW * 8];
+    float* const ml = (float*)(lds + NW * SLICE);           // [wave][query][2]
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -140,10 +144,15 @@ __global__ void __launch_bounds__(NWAVES * 64, 2) attn_kv8_kernel(const Kv8Attn 
         const int nt = gridDim.x, bid = blockIdx.x;
         const int xcd = bid & 7, per = nt >> 3, rem = nt & 7;
         int item = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (bid >> 3);
-        qb = item % a.n_qblocks;
-        item /= a.n_qblocks;
-        ks = item % a.splits;
-        item /= a.splits;
+        qb = ks = 0;
+        if (a.n_qblocks > 1) {
+            qb = item % a.n_qblocks;
+            item /= a.n_qblocks;
+        }
+        if (a.splits > 1) {
+            ks = item % a.splits;
+            item /= a.splits;
+        }
         h = item % a.n_heads;
         b = item / a.n_heads;
     }
@@ -171,11 +180,14 @@ __global__ void __launch_bounds__(NWAVES * 64, 2) attn_kv8_kernel(const Kv8Attn 
     w.m = -INFINITY;
     w.l = 0.f;
 
-    const int u_end = min(a.n_units, (ks + 1) * a.per_split);
-    int u = ks * a.per_split + kg;
+    // units of this workgroup: [u_begin, u_end) of the fresh tiles, then the cached ones; unit u_begin + i is key group i % NK's
+    const int n_fresh = a.n_units - a.n_cached;
+    const int u_begin = ks * a.per_split, u_end = min(a.n_units, u_begin + a.per_split);
+    const int c_begin = max(u_begin, n_fresh);
+    int u = c_begin + ((kg - (c_begin - u_begin)) & (NK - 1));          // this wave's first cached one
 
-    // ---- cached tiles ----
-    auto tile_of = [&](int i) { return i < a.skip_from ? i : i + a.skipped; };
+    // The first cached tile's keys are fetched ahead of everything else.
+    auto tile_of = [&](int i) { i -= n_fresh; return i < a.skip_from ? i : i + a.skipped; };
     u32x4 kc[8], vc[8];
     auto load_keys = [&](int t) {
 #pragma unroll
@@ -192,141 +204,185 @@ __global__ void __launch_bounds__(NWAVES * 64, 2) attn_kv8_kernel(const Kv8Attn 
     };
     auto mask_byte = [&](int t) -> uint8_t { return mask ? mask[min(t * KV8_TOKENS + lane, a.seq_len - 1)] : (uint8_t)1; };
 
-    const int c_end = min(u_end, a.n_cached);
-    if (u < c_end) {
-        int t = tile_of(u);
+    int t = 0;
+    uint8_t mb = 0;
+    float ks_next = 1.f, vs_next = 1.f;
+    if (u < u_end) {
+        t = tile_of(u);
         load_keys(t);
-        load_values(t);
-        uint8_t mb = mask_byte(t);
-        float ks_next = scales[2 * t], vs_next = scales[2 * t + 1];
-        for (; u < c_end; u += NK) {
-            const uint64_t valid = live_keys(t, mb);
-            const float kscale = ks_next, vscale = vs_next;
-            const int tn = u + NK < c_end ? tile_of(u + NK) : t;      // (the last tile is fetched once more and dropped)
+        mb = mask_byte(t);
+        ks_next = scales[2 * t];
+        vs_next = scales[2 * t + 1];
+    }
+
+    // Fresh tiles are bf16 rows, and rows of values have to be read transposed: they cross the LDS, which the cached tiles leave
+    // idle.  They come first, while the first cached tile is on its way.  All waves bring them in by LDS-DMA, keys and values of two tiles at a time (a query group's whole sweep: the
+    // next tile under the work on this one; several key groups: a round of two, a tile for each of two groups).
+    // 16-byte chunk c of key row k stands at c ^ (k & 15), 64-byte slot s of value row k at s ^ (k & 3): applied to the
+    // source address, so that no read meets a bank twice.
+    constexpr int FRESH = 2 * KV8_TOKENS * 256;                         // bytes of a tile
+    constexpr int AHEAD = NK == 1 ? 1 : 2;                              // tiles of a round
+    static_assert(2 * FRESH <= NW * SLICE, "two tiles fit the slices");
+    auto fetch_fresh = [&](int f, int buf) {
+        const bf16_t* const rows = a.blk + (size_t)b * a.blk_len * (size_t)a.blk_stride + h * KV8_HD + d;
+        const int f0 = f * KV8_TOKENS, row0 = lane >> 4, at = lane & 15;
+#pragma unroll
+        for (int i = 0; i < 32 / NW; ++i) {
+            const int piece = wave + i * NW, is_v = piece >> 4;         // 0 .. 15: four key rows each, 16 .. 31: value rows
+            const int row = (piece & 15) * 4 + row0;
+            const int chunk = is_v ? ((((at >> 2) ^ (row & 3)) << 2) | (at & 3)) : (at ^ (row & 15));
+            const bf16_t* src = rows + (is_v ? d : 0) + (size_t)min(f0 + row, a.blk_len - 1) * (size_t)a.blk_stride + chunk * 8;
+            __builtin_amdgcn_global_load_lds((gbl_void_ptr)src, (lds_void_ptr)(lds + buf * FRESH + piece * 1024), 16, 0, 0);
+        }
+    };
+    const int f_end = min(u_end, n_fresh);
+    int f_next = u_begin;                                               // first fresh tile of the next round
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (f_next + i < f_end) fetch_fresh(f_next + i, i);
+    for (int buf = 0; f_next < f_end; f_next += AHEAD) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // this wave's pieces have landed
+        __syncthreads();                                                // everyone's
+        const int f = NK == 1 ? f_next : f_next + ((kg + u_begin - f_next) & (NK - 1));     // the tile of this round that is this wave's
+        const int f0 = f * KV8_TOKENS;
+        if (NK == 1 && f + 1 < f_end) fetch_fresh(f + 1, buf ^ 1);      // (the buffer of the last round is no longer read)
+        if (f < min(f_next + AHEAD, f_end)) {
+            unsigned char* const k_lds = lds + (NK == 1 ? buf : f - f_next) * FRESH;
+            unsigned char* const v_lds = k_lds + KV8_TOKENS * 256;
+            const int fk = f0 + lane;
+            const uint64_t there = a.blk_len - f0 >= 64 ? ~0ull : (1ull << (a.blk_len - f0)) - 1;
+            const uint64_t unmasked = __builtin_amdgcn_ballot_w64(mask == nullptr || fk >= a.blk_len || mask[min(a.blk_start + fk, a.seq_len - 1)] != 0);
+            if ((unmasked & there) != there) {                          // what stands under a masked token, and the copies of
+                                                                        // the last row behind the block: zeros
+                // (waves of several query groups write the same zeros to a tile of theirs, each before its own reads)
+#pragma unroll
+                for (int i = 0; i < KV8_TOKENS / 4; ++i)
+                    if (!(((unmasked & there) >> (i * 4 + (lane >> 4))) & 1)) *(u32x4*)(v_lds + i * 1024 + lane * 16) = (u32x4){0u, 0u, 0u, 0u};
+            }
             f32x16 s[2];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-                        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            codes_to_bf16<TYPE>(kc[kb * 4 + j][2 * half], kc[kb * 4 + j][2 * half + 1]), qf[2 * j + half], s[kb], 0, 0, 0);
-            load_keys(tn);
-            mb = mask_byte(tn);
-            ks_next = scales[2 * tn];
-            vs_next = scales[2 * tn + 1];
-            bf16x8 pb[2][2];
-            const float ve = (float)((int)(__float_as_uint(vscale) >> 23) - 127);
-            softmax_tile(s, valid, a.scale_log2e * kscale, ve, __uint_as_float((254u << 23) - __float_as_uint(vscale)), w, pb, hg);
-            if (valid != ~0ull) {          // zero codes under masked keys: 0 * NaN would reach the sums
-                const uint64_t mine = valid >> (4 * hg);
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const unsigned nib = (unsigned)(mine >> (kb * 32 + 8 * i)) & 15u;
-                        const unsigned keep = ((nib * 0x00204081u) & 0x01010101u) * 255u;
-#pragma unroll
-                        for (int db = 0; db < 4; ++db) vc[db * 2 + kb][i] &= keep;
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const bf16x8 kf = *(const bf16x8*)(k_lds + (kb * 32 + r) * 256 + (((8 * hg + i) ^ (r & 15)) * 16));
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i], s[kb], 0, 0, 0);
+                }
             }
+            bf16x8 pb[2][2];
+            softmax_tile(s, unmasked & there, a.scale_log2e, 0.f, 1.f, w, pb, hg);
+            const int q4 = (lane & 15) >> 2, p4 = lane & 3, g1 = (lane >> 4) & 1;
+            const unsigned char* const vrow = v_lds + (4 * hg + q4) * 256 + 32 * g1 + 8 * p4;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int ss = 0; ss < 2; ++ss)
 #pragma unroll
-                    for (int db = 0; db < 4; ++db)
-                        w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            codes_to_bf16<TYPE>(vc[db * 2 + kb][2 * ss], vc[db * 2 + kb][2 * ss + 1]), pb[kb][ss], w.o[db], 0, 0, 0);
-            load_values(tn);
-            t = tn;
+                    for (int db = 0; db < 4; ++db) {
+                        const unsigned char* p = vrow + (kb * 32 + 16 * ss) * 256 + ((db * 64) ^ (q4 * 64));
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p);
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 8 * 256));
+                        const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                        w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pb[kb][ss], w.o[db], 0, 0, 0);
+                    }
+        }
+        if constexpr (NK == 1) {
+            buf ^= 1;
+        } else if (f_next + AHEAD < f_end) {
+            __syncthreads();                                            // both tiles have been read
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (f_next + AHEAD + i < f_end) fetch_fresh(f_next + AHEAD + i, i);
         }
     }
-
-    // ---- fresh tiles: bf16 rows; the values cross the wave's LDS slice to be read transposed ----
-    unsigned char* const slice = lds + wave * SLICE;
+    // ---- cached tiles ----
+    if (u < u_end) load_values(t);
     for (; u < u_end; u += NK) {
-        const int f0 = (u - a.n_cached) * KV8_TOKENS;                   // first row of the tile inside the block
-        const bf16_t* const rows = a.blk + (size_t)b * a.blk_len * (size_t)a.blk_stride + h * KV8_HD + d;
-        const int fk = f0 + lane;
-        const uint8_t fm = mask && fk < a.blk_len ? mask[a.blk_start + fk] : (uint8_t)1;
-        const uint64_t valid = __builtin_amdgcn_ballot_w64(fk < a.blk_len && fm != 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int row = i * 4 + (lane >> 4), c = lane & 15;
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if ((valid >> row) & 1) v = *(const u32x4*)(rows + d + (size_t)(f0 + row) * (size_t)a.blk_stride + c * 8);
-            *(u32x4*)(slice + row * 256 + (((c >> 2) ^ (row & 3)) << 6) + (c & 3) * 16) = v;
-        }
+        const uint64_t valid = live_keys(t, mb);
+        const float kscale = ks_next, vscale = vs_next;
+        const int tn = u + NK < u_end ? tile_of(u + NK) : t;      // (the last tile is fetched once more and dropped)
         f32x16 s[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-            const bf16_t* kp = rows + (size_t)min(f0 + kb * 32 + r, a.blk_len - 1) * (size_t)a.blk_stride + hg * 64;
-            bf16x8 kf[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) kf[i] = *(const bf16x8*)(kp + i * 8);
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i], qf[i], s[kb], 0, 0, 0);
-        }
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        codes_to_bf16<TYPE>(kc[kb * 4 + j][2 * half], kc[kb * 4 + j][2 * half + 1]), qf[2 * j + half], s[kb], 0, 0, 0);
+        load_keys(tn);
+        mb = mask_byte(tn);
+        ks_next = scales[2 * tn];
+        vs_next = scales[2 * tn + 1];
         bf16x8 pb[2][2];
-        softmax_tile(s, valid, a.scale_log2e, 0.f, 1.f, w, pb, hg);
-        const int q4 = (lane & 15) >> 2, p4 = lane & 3, g1 = (lane >> 4) & 1;
-        const unsigned char* const vrow = slice + (4 * hg + q4) * 256 + 32 * g1 + 8 * p4;
+        const float ve = (float)((int)(__float_as_uint(vscale) >> 23) - 127);
+        softmax_tile(s, valid, a.scale_log2e * kscale, ve, __uint_as_float((254u << 23) - __float_as_uint(vscale)), w, pb, hg);
+        if (valid != ~0ull) {          // zero codes under masked keys: 0 * NaN would reach the sums
+            const uint64_t mine = valid >> (4 * hg);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned nib = (unsigned)(mine >> (kb * 32 + 8 * i)) & 15u;
+                    const unsigned keep = ((nib * 0x00204081u) & 0x01010101u) * 255u;
+#pragma unroll
+                    for (int db = 0; db < 4; ++db) vc[db * 2 + kb][i] &= keep;
+                }
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int ss = 0; ss < 2; ++ss)
 #pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    const unsigned char* p = vrow + (kb * 32 + 16 * ss) * 256 + ((db * 64) ^ (q4 * 64));
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p);
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 8 * 256));
-                    const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pb[kb][ss], w.o[db], 0, 0, 0);
-                }
+                for (int db = 0; db < 4; ++db)
+                    w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        codes_to_bf16<TYPE>(vc[db * 2 + kb][2 * ss], vc[db * 2 + kb][2 * ss + 1]), pb[kb][ss], w.o[db], 0, 0, 0);
+        load_values(tn);
+        t = tn;
     }
 
-    // ---- the key groups' results, rescaled to their common maximum, are summed out of LDS ----
+    unsigned char* const slice = lds + wave * SLICE;
+
+    // ---- the key groups' results meet in LDS and are summed at their common maximum ----
     const float l_tot = w.l + __shfl_xor(w.l, 32);
+    if (f_end > u_begin) __syncthreads();                               // the fresh tiles have been read
     if (hg == 0) {
         ml[(wave * QW + r) * 2] = w.m;
         ml[(wave * QW + r) * 2 + 1] = l_tot;
     }
-    __syncthreads();
-    float m_all = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < NK; ++k) m_all = fmaxf(m_all, ml[((k * NQ + qg) * QW + r) * 2]);
-    const float f = __builtin_amdgcn_exp2f(w.m - (m_all == -INFINITY ? 0.f : m_all));
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             *(f32x4*)(slice + r * OROW + (db * 32 + 8 * c + 4 * hg) * 4) =
-                (f32x4){w.o[db][4 * c] * f, w.o[db][4 * c + 1] * f, w.o[db][4 * c + 2] * f, w.o[db][4 * c + 3] * f};
+                (f32x4){w.o[db][4 * c], w.o[db][4 * c + 1], w.o[db][4 * c + 2], w.o[db][4 * c + 3]};
     __syncthreads();
     // wave kg of a query group writes 32 / NK of its queries: 16 lanes a row, 8 dims a lane
 #pragma unroll
     for (int i = 0; i < QW / NK / 4; ++i) {
         const int row = kg * (QW / NK) + i * 4 + (lane >> 4), c = lane & 15;
-        float mr = -INFINITY, lr = 0.f;
+        float m[NK], l[NK], mr = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < NK; ++k) mr = fmaxf(mr, ml[((k * NQ + qg) * QW + row) * 2]);
+        for (int k = 0; k < NK; ++k) {
+            m[k] = ml[((k * NQ + qg) * QW + row) * 2];
+            l[k] = ml[((k * NQ + qg) * QW + row) * 2 + 1];
+            mr = fmaxf(mr, m[k]);
+        }
         const float mu = mr == -INFINITY ? 0.f : mr;
+        float lr = 0.f;
         f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
-            const int wv = k * NQ + qg;
-            lr += ml[(wv * QW + row) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(wv * QW + row) * 2] - mu);
-            const unsigned char* p = lds + wv * SLICE + row * OROW + c * 32;
-            x0 += *(const f32x4*)p;
-            x1 += *(const f32x4*)(p + 16);
+            const float f = __builtin_amdgcn_exp2f(m[k] - mu);
+            const unsigned char* p = lds + (k * NQ + qg) * SLICE + row * OROW + c * 32;
+            lr += l[k] * f;
+            x0 += *(const f32x4*)p * f;
+            x1 += *(const f32x4*)(p + 16) * f;
         }
         const int q = q0 + row;
         if (q >= a.n_q) continue;
@@ -382,41 +438,66 @@ __global__ void __launch_bounds__(256) attn_kv8_combine_kernel(const float* __re
 
 constexpr int MAX_SPLITS = 16;
 
-// Key splits of a launch of `wgs` workgroups over `units` tiles: up to about 512 workgroups (two per CU), none with
-// fewer than two tiles for each of its key groups.
-int pick_splits(int64_t wgs, int units, int nk) {
-    if (wgs >= 256) return 1;
-    int64_t s = 512 / wgs;
-    const int most = units / (2 * nk);
-    s = s < most ? s : most;
-    s = s < MAX_SPLITS ? s : MAX_SPLITS;
-    return s < 1 ? 1 : (int)s;
-}
+int g_force_nq = 0, g_force_splits = 0;     // test hook: 0 = automatic
 
-int query_groups(int n_q) { return n_q <= 32 ? 1 : n_q <= 64 ? 2 : 4; }
+struct Plan {
+    int nq, splits;
+};
+
+// How a call's queries and tiles are dealt to waves (measured; times in us, 32 heads).
+Plan pick_plan(int64_t n_seq, int n_q, int n_heads, int units, bool scratch) {
+    auto workgroups = [&](int nq) { return (int64_t)((n_q + nq * QW - 1) / (nq * QW)) * n_heads * n_seq; };
+    Plan p;
+    // Waves that hold different queries share a tile's fetch; waves that share the queries fill more CUs.  The former while
+    // every CU still has a workgroup: 64 x 640 tokens, 64 queries: 2 groups 94, 1 group 108; 4 x 2048, 128 queries: 2 groups
+    // (256 workgroups) 25, 4 groups (128) 35.
+    p.nq = 1;
+    while (p.nq < 4 && n_q > p.nq * QW && workgroups(2 * p.nq) >= 256) p.nq *= 2;
+    if (g_force_nq) p.nq = g_force_nq;
+    p.splits = 1;
+    if (!scratch) return p;
+    // Key splits cost a second launch and a round trip of float32 partial results: up to one workgroup per CU, 16 tiles
+    // each at least.  One sequence, 32 queries, unsplit / split: 1150 tokens 10.3 / 11.1, 2048: 14.5 / 14.0 (2 splits),
+    // 4096: 21.6 / 15.4 (4); 4 sequences of 16384: 116 / 98 (2), 112 (4).
+    const int64_t wgs = workgroups(p.nq);
+    if (g_force_splits) {
+        p.splits = g_force_splits < units ? g_force_splits : units;
+    } else if (wgs <= 128) {
+        const int64_t s = 256 / wgs;
+        const int most = units / 16;
+        p.splits = s < most ? (int)s : most > 1 ? most : 1;
+    }
+    if (p.splits > MAX_SPLITS) p.splits = MAX_SPLITS;
+    return p;
+}
 
 size_t part_bytes(int64_t n_rows, int n_heads, int splits) {
     return (size_t)splits * n_rows * ((size_t)n_heads * KV8_HD * 4 + (size_t)n_heads * 8);
 }
 
 template <int TYPE>
-void launch(const Kv8Attn& a, int nq, unsigned grid, hipStream_t st) {
-    if (nq == 1)
-        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 1>), dim3(grid), dim3(NWAVES * 64), 0, st, a);
-    else if (nq == 2)
-        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 2>), dim3(grid), dim3(NWAVES * 64), 0, st, a);
+void launch(const Kv8Attn& a, Plan p, unsigned grid, hipStream_t st) {
+    if (p.nq == 1)
+        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 1>), dim3(grid), dim3(NW * 64), 0, st, a);
+    else if (p.nq == 2)
+        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 2>), dim3(grid), dim3(NW * 64), 0, st, a);
     else
-        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 4>), dim3(grid), dim3(NWAVES * 64), 0, st, a);
+        hipLaunchKernelGGL((attn_kv8_kernel<TYPE, 4>), dim3(grid), dim3(NW * 64), 0, st, a);
 }
 
 }  // namespace
 
 extern "C" size_t llada_attn_kv8_workspace_bytes(int32_t n_seq, int32_t n_q, int32_t seq_len, int32_t n_heads) {
     if (n_seq <= 0 || n_q <= 0 || seq_len <= 0 || n_heads <= 0) return 0;
-    const int nq = query_groups(n_q);
-    const int64_t wgs = (int64_t)((n_q + nq * QW - 1) / (nq * QW)) * n_heads * n_seq;
-    const int splits = pick_splits(wgs, (int)kv8_blocks(seq_len) + 1, NWAVES / nq);     // + 1: a fresh block cut by tile borders
-    return splits > 1 ? part_bytes((int64_t)n_seq * n_q, n_heads, splits) : 0;
+    // + 1: a fresh block that tile borders cut sweeps one tile more
+    const Plan p = pick_plan(n_seq, n_q, n_heads, (int)kv8_blocks(seq_len) + 1, true);
+    return p.splits > 1 ? part_bytes((int64_t)n_seq * n_q, n_heads, p.splits) : 0;
+}
+
+// tests and sweeps: query groups of a workgroup (1, 2, 4), key splits; 0 = automatic
+extern "C" void llada_attn_kv8_force(int nq, int splits) {
+    g_force_nq = nq;
+    g_force_splits = splits;
 }
 
 extern "C" int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, const void* cache, int32_t kv_type,
@@ -469,10 +550,10 @@ extern "C" int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, cons
     }
     a.n_cached = (int)n_blocks - a.skipped;
     a.n_units = a.n_cached + fresh;
-    const int nq = query_groups(n_q);
-    a.n_qblocks = (n_q + nq * QW - 1) / (nq * QW);
+    const Plan plan = pick_plan(n_seq, n_q, n_heads, a.n_units, workspace != nullptr);
+    a.n_qblocks = (n_q + plan.nq * QW - 1) / (plan.nq * QW);
     const int64_t wgs = (int64_t)a.n_qblocks * n_heads * n_seq;
-    int splits = workspace ? pick_splits(wgs, a.n_units, NWAVES / nq) : 1;
+    int splits = plan.splits;
     while (splits > 1 && part_bytes(a.n_rows, n_heads, splits) > workspace_bytes) --splits;
     a.per_split = (a.n_units + splits - 1) / splits;
     a.splits = (a.n_units + a.per_split - 1) / a.per_split;             // no empty run
@@ -482,9 +563,9 @@ extern "C" int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, cons
                           "attn_kv8: grid too large");
     hipStream_t st = (hipStream_t)stream;
     if (kv_type == LLADA_KV_E4M3)
-        launch<LLADA_KV_E4M3>(a, nq, (unsigned)(wgs * a.splits), st);
+        launch<LLADA_KV_E4M3>(a, plan, (unsigned)(wgs * a.splits), st);
     else
-        launch<LLADA_KV_INT8>(a, nq, (unsigned)(wgs * a.splits), st);
+        launch<LLADA_KV_INT8>(a, plan, (unsigned)(wgs * a.splits), st);
     LLADA_CHECK_LAUNCH("attn_kv8_kernel");
     if (a.splits > 1) {
         const int64_t items = a.n_rows * n_heads * (KV8_HD / 4);

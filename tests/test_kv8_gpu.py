@@ -322,3 +322,16 @@ def test_captured_step_on_a_side_stream(lib):
         assert torch.equal(out, want)
         assert torch.equal(after[0], e.read(0)[0]) and torch.equal(after[1], e.read(0)[1])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("nq", [1, 2, 4])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("n_q,start,fresh", [(20, 100, True), (75, 300, True), (150, 0, True), (260, 140, True), (33, 0, False)])
+def test_every_way_to_deal_the_work(lib, nq, splits, n_q, start, fresh):
+    """Query groups and key splits forced: the bound holds whatever the plan (fresh tiles in one split, in several, in none)."""
+    n, L, H = 2, 400, 2
+    try:
+        lib.llada_attn_kv8_force(nq, splits)
+        check_attend(make(n, L, H, "e4m3"), rows(L + nq, n, L, H), H, n_q, "e4m3", left_mask(n, L, n_q), fresh, start)
+    finally:
+        lib.llada_attn_kv8_force(0, 0)
