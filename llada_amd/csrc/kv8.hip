@@ -28,30 +28,31 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 
 __device__ __forceinline__ float power_of_two(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }
 
-__device__ __forceinline__ float finite_abs(float x) {
-    const float a = fabsf(x);
-    return a < INFINITY ? a : 0.f;
-}
-
-// four values -> four codes
-template <int TYPE>
+// Four values -> four codes.  RAW: all four are finite (then |x inv| is within the code's range by the choice of the scale).
+template <int TYPE, bool RAW>
 __device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv) {
-    float y[4] = {a * inv, b * inv, c * inv, d * inv};
+    float x[4] = {a, b, c, d};
     if constexpr (TYPE == LLADA_KV_E4M3) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = y[i] != y[i] ? y[i] : __builtin_amdgcn_fmed3f(y[i], -448.f, 448.f);
+        for (int i = 0; i < 4; ++i) {
+            x[i] *= inv;
+            if (!RAW) x[i] = x[i] != x[i] ? x[i] : __builtin_amdgcn_fmed3f(x[i], -448.f, 448.f);
+        }
         int r = 0;
-        r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], r, false);
-        r = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], r, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
         return (unsigned)r;
     } else {
-        unsigned r = 0;
+        // 1.5 * 2^23 + y: the sum's last bit stands for 1, so the addition rounds y to the nearest integer, ties to even,
+        // and leaves it in two's complement in the low byte (x inv is exact: one rounding)
+        unsigned u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int v = y[i] != y[i] ? 0 : (int)__builtin_rintf(__builtin_amdgcn_fmed3f(y[i], -127.f, 127.f));
-            r |= (unsigned)(v & 255) << (8 * i);
+            if (!RAW) x[i] = x[i] != x[i] ? 0.f : __builtin_amdgcn_fmed3f(x[i] * inv, -127.f, 127.f);
+            u[i] = __float_as_uint(RAW ? __builtin_fmaf(x[i], inv, 12582912.f) : x[i] + 12582912.f);
         }
-        return r;
+        const unsigned lo = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0400u);
+        return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
     }
 }
 
@@ -69,9 +70,33 @@ __device__ __forceinline__ float decode(unsigned word, int byte) {
     }
 }
 
+// entry e (0 .. 7) of four words of bf16 pairs
+__device__ __forceinline__ float entry(u32x4 w, int e) { return __uint_as_float((e & 1) ? (w[e >> 1] & 0xFFFF0000u) : (w[e >> 1] << 16)); }
+
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+__device__ __forceinline__ u16x2 halves(unsigned w) { return __builtin_bit_cast(u16x2, w); }
+
+// x: four keys x 8 dims of the keys and of the values; their codes into the tile's LDS image.
+template <int TYPE, bool RAW>
+__device__ __forceinline__ void encode_tile(const u32x4 (&x)[2][4], float ik, float iv, unsigned char* codes, int kg, int dg) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        u32x2 w;
+        w[0] = encode4<TYPE, RAW>(entry(x[0][i], 0), entry(x[0][i], 1), entry(x[0][i], 2), entry(x[0][i], 3), ik);
+        w[1] = encode4<TYPE, RAW>(entry(x[0][i], 4), entry(x[0][i], 5), entry(x[0][i], 6), entry(x[0][i], 7), ik);
+        *(u32x2*)(codes + kv8_key_offset(kg * 4 + i, dg * 8)) = w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        *(unsigned*)(codes + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e)) =
+            encode4<TYPE, RAW>(entry(x[1][0], e), entry(x[1][1], e), entry(x[1][2], e), entry(x[1][3], e), iv);
+}
+
 // One workgroup = one (sequence, head, block): thread (kg, dg) holds keys 4 kg .. + 3 and dims 8 dg .. + 7 of the keys
-// and of the values (two whole 256-byte head rows per four threads of loads).  Bound by memory: 4 bytes in and 2 out
-// per channel; the codes cross the LDS once to leave as whole 1-KiB runs.
+// and of the values, as bf16 pairs (what a cache holds is exact in bf16).  Bound by memory, 4 bytes in and 2 out per
+// channel, once the arithmetic is out of its way: the largest magnitude is taken on packed 16-bit patterns (2
+// instructions for two elements), and a block without infinities and NaNs, known from that maximum, needs no clamp: under
+// three instructions an element.  The codes cross the LDS once to leave as whole 1-KiB runs.
 template <int TYPE>
 __global__ void __launch_bounds__(THREADS) kv8_write_kernel(const bf16_t* __restrict__ rows, int64_t row_stride,
                                                             const uint8_t* __restrict__ key_mask, float* __restrict__ scales,
@@ -79,92 +104,101 @@ __global__ void __launch_bounds__(THREADS) kv8_write_kernel(const bf16_t* __rest
                                                             int n_blocks, int start, int len, int first_block,
                                                             int touched) {
     __shared__ __attribute__((aligned(16))) unsigned char codes[KV8_TILE];
-    __shared__ float red[2][THREADS / 64];
+    __shared__ unsigned red[2][THREADS / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int kg = tid >> 4, dg = tid & 15;
-    int64_t item = blockIdx.x;
-    const int h = (int)(item % n_heads);
-    item /= n_heads;
-    const int t = first_block + (int)(item % touched);
-    const int b = (int)(item / touched);
+    unsigned item = blockIdx.x;
+    const int h = (int)(item % (unsigned)n_heads);
+    item /= (unsigned)n_heads;
+    const int t = first_block + (int)(item % (unsigned)touched);
+    const int b = (int)(item / (unsigned)touched);
     const int64_t tile = ((int64_t)b * n_heads + h) * n_blocks + t;
     unsigned char* const dst = tiles + (size_t)tile * KV8_TILE;
     float* const sc = scales + tile * 2;
     const int d = n_heads * KV8_HD;
     const int key0 = t * KV8_TOKENS + kg * 4;
+    const int t_end = min(seq_len, (t + 1) * KV8_TOKENS);
+    const bool partial = start > t * KV8_TOKENS || start + len < t_end;      // (uniform)
 
-    float x[2][4][8];                    // keys, values
-    bool old[4];                         // a token outside the range that stays: taken as the cache holds it
+    // every load first: rows clamped into the range, what does not count is replaced below
+    u32x4 x[2][4];
+    uint8_t m[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int key = key0 + i;
-        const bool live = key < seq_len && (key_mask == nullptr || key_mask[(size_t)b * seq_len + key] != 0);
-        const bool fresh = key >= start && key < start + len;
-        old[i] = live && !fresh;
-        u32x4 w[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
-        if (live && fresh) {
-            const bf16_t* p = rows + ((size_t)b * len + (key - start)) * row_stride + d + h * KV8_HD + dg * 8;
-            w[0] = *(const u32x4*)p;
-            w[1] = *(const u32x4*)(p + d);
-        }
-#pragma unroll
-        for (int o = 0; o < 2; ++o)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[o][i][e] = __uint_as_float((e & 1) ? (w[o][e >> 1] & 0xFFFF0000u) : (w[o][e >> 1] << 16));
+        const int row = min(max(key0 + i - start, 0), len - 1);
+        const bf16_t* p = rows + ((size_t)b * len + row) * row_stride + d + h * KV8_HD + dg * 8;
+        x[0][i] = __builtin_nontemporal_load((const u32x4*)p);
+        x[1][i] = __builtin_nontemporal_load((const u32x4*)(p + d));
+        m[i] = key_mask ? key_mask[(size_t)b * seq_len + min(key0 + i, seq_len - 1)] : (uint8_t)1;
     }
-    // a block that the range covers only in part: its other tokens as the cache holds them (uniform branch)
-    const int t_end = min(seq_len, (t + 1) * KV8_TOKENS);
-    if (start > t * KV8_TOKENS || start + len < t_end) {
+    if (partial) {       // the block's other tokens as the cache holds them
         const float sk = sc[0], sv = sc[1];
+        u32x2 kw[4];
+        unsigned vw[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const unsigned vw = *(const unsigned*)(dst + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e));
+        for (int i = 0; i < 4; ++i) kw[i] = *(const u32x2*)(dst + kv8_key_offset(kg * 4 + i, dg * 8));
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (old[i]) x[1][i][e] = decode<TYPE>(vw, i) * sv;
-        }
+        for (int e = 0; e < 8; ++e) vw[e] = *(const unsigned*)(dst + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (old[i]) {
-                const u32x2 kw = *(const u32x2*)(dst + kv8_key_offset(kg * 4 + i, dg * 8));
+            const int key = key0 + i;
+            if (key >= start && key < start + len) continue;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[0][i][e] = decode<TYPE>(kw[e >> 2], e & 3) * sk;
+            for (int w = 0; w < 4; ++w) {
+                x[0][i][w] = pack_bf16x2(decode<TYPE>(kw[i][w >> 1], (2 * w) & 3) * sk, decode<TYPE>(kw[i][w >> 1], (2 * w + 1) & 3) * sk);
+                x[1][i][w] = pack_bf16x2(decode<TYPE>(vw[2 * w], i) * sv, decode<TYPE>(vw[2 * w + 1], i) * sv);
             }
         }
     }
-
-    float amax[2] = {0.f, 0.f};
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
+    for (int i = 0; i < 4; ++i)
+        if (key0 + i >= seq_len || m[i] == 0) x[0][i] = x[1][i] = (u32x4){0u, 0u, 0u, 0u};
+
+    // largest magnitude of the block: of all patterns first, of the finite ones where that is not finite
+    auto largest = [&](bool finite_only, int o) {
+        u16x2 most = {0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) amax[o] = fmaxf(amax[o], finite_abs(x[o][i][e]));
-        amax[o] = wave_reduce_max(amax[o]);
-        if (lane == 0) red[o][wave] = amax[o];
+            for (int w = 0; w < 4; ++w) {
+                u16x2 a = halves(x[o][i][w] & 0x7FFF7FFFu);
+                if (finite_only) a = (u16x2){a[0] < 0x7F80 ? a[0] : (unsigned short)0, a[1] < 0x7F80 ? a[1] : (unsigned short)0};
+                most = __builtin_elementwise_max(most, a);
+            }
+        unsigned v = most[0] > most[1] ? most[0] : most[1];
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) {
+            const unsigned u = (unsigned)__shfl_xor((int)v, s);
+            v = v > u ? v : u;
+        }
+        return v;
+    };
+    auto block_largest = [&](bool finite_only, unsigned (&out)[2]) {
+        const unsigned a = largest(finite_only, 0), c = largest(finite_only, 1);
+        if (lane == 0) {
+            red[0][wave] = a;
+            red[1][wave] = c;
+        }
+        __syncthreads();                 // also: every old code of this tile has been read
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            out[o] = red[o][0];
+#pragma unroll
+            for (int w = 1; w < THREADS / 64; ++w) out[o] = out[o] > red[o][w] ? out[o] : red[o][w];
+        }
+    };
+    unsigned most[2];
+    block_largest(false, most);
+    const bool raw = most[0] < 0x7F80u && most[1] < 0x7F80u;      // (uniform)
+    if (!raw) {
+        __syncthreads();
+        block_largest(true, most);
     }
-    __syncthreads();                     // also: every old code of this tile has been read
-    int k[2];
-#pragma unroll
-    for (int o = 0; o < 2; ++o) {
-        float m = red[o][0];
-#pragma unroll
-        for (int w = 1; w < THREADS / 64; ++w) m = fmaxf(m, red[o][w]);
-        k[o] = scale_exponent<TYPE>(m);
-    }
-    const float ik = power_of_two(-k[0]), iv = power_of_two(-k[1]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        u32x2 w;
-        w[0] = encode4<TYPE>(x[0][i][0], x[0][i][1], x[0][i][2], x[0][i][3], ik);
-        w[1] = encode4<TYPE>(x[0][i][4], x[0][i][5], x[0][i][6], x[0][i][7], ik);
-        *(u32x2*)(codes + kv8_key_offset(kg * 4 + i, dg * 8)) = w;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        *(unsigned*)(codes + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e)) =
-            encode4<TYPE>(x[1][0][e], x[1][1][e], x[1][2][e], x[1][3][e], iv);
+    const int k[2] = {scale_exponent<TYPE>(__uint_as_float(most[0] << 16)), scale_exponent<TYPE>(__uint_as_float(most[1] << 16))};
+    if (raw)
+        encode_tile<TYPE, true>(x, power_of_two(-k[0]), power_of_two(-k[1]), codes, kg, dg);
+    else
+        encode_tile<TYPE, false>(x, power_of_two(-k[0]), power_of_two(-k[1]), codes, kg, dg);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < KV8_TILE / (16 * THREADS); ++i) {
@@ -181,11 +215,11 @@ __global__ void __launch_bounds__(THREADS) kv8_read_kernel(const float* __restri
                                                            bf16_t* __restrict__ v_out, int seq_len, int n_heads, int n_blocks) {
     __shared__ __attribute__((aligned(16))) unsigned char codes[KV8_TILE];
     const int tid = threadIdx.x, kg = tid >> 4, dg = tid & 15;
-    int64_t item = blockIdx.x;
-    const int h = (int)(item % n_heads);
-    item /= n_heads;
-    const int t = (int)(item % n_blocks);
-    const int b = (int)(item / n_blocks);
+    unsigned item = blockIdx.x;
+    const int h = (int)(item % (unsigned)n_heads);
+    item /= (unsigned)n_heads;
+    const int t = (int)(item % (unsigned)n_blocks);
+    const int b = (int)(item / (unsigned)n_blocks);
     const int64_t tile = ((int64_t)b * n_heads + h) * n_blocks + t;
     const unsigned char* const src = tiles + (size_t)tile * KV8_TILE;
     const float sk = scales[tile * 2], sv = scales[tile * 2 + 1];
@@ -210,8 +244,8 @@ __global__ void __launch_bounds__(THREADS) kv8_read_kernel(const float* __restri
             c[w] = pack_bf16x2(decode<TYPE>(vw[2 * w], i) * sv, decode<TYPE>(vw[2 * w + 1], i) * sv);
         }
         const size_t at = ((size_t)b * seq_len + key) * ((size_t)n_heads * KV8_HD) + (size_t)h * KV8_HD + dg * 8;
-        *(u32x4*)(k_out + at) = a;
-        *(u32x4*)(v_out + at) = c;
+        __builtin_nontemporal_store(a, (u32x4*)(k_out + at));
+        __builtin_nontemporal_store(c, (u32x4*)(v_out + at));
     }
 }
 
