@@ -67,30 +67,17 @@ struct Shared {
     int irregular;
     int j, tied;                     // the drawn entry: the j-th of `tied` equal ones
     float value, prob;
-    unsigned slot_tot[SLOTS];
+    unsigned slot_tot[SLOTS / 2];    // two slots a word
     unsigned wave_tot[NWV];
     int token;
-    unsigned short keys[REGULAR_KEYS + 64];   // regular rows: the keys that have entries, in order
+    unsigned short patterns[REGULAR_KEYS + 64];   // regular rows: the values that have entries, in order
 };
 static_assert(REST_AT * 4 + sizeof(Shared) <= NEGATIVE * 4 && LDS_WORDS * 4 <= 160 * 1024, "the planes leave room");
 
-// Key s of a row's value order (0 = the largest) <-> value.  Regular rows: the histogram's own order; irregular rows: all
-// bf16 patterns.
-__device__ __forceinline__ float key_value(int s, bool regular) {
-    if (regular) {
-        if (s == SPAN) return 0.f;
-        return s < SPAN ? __uint_as_float((MAG_HI - 1 - s) << 16)
-                        : __uint_as_float(0x80000000u | ((MAG_LO + (s - SPAN - 1)) << 16));
-    }
-    const unsigned k = 65535u - (unsigned)s;
-    return __uint_as_float(((k & 0x8000u) ? k ^ 0x8000u : ~k & 0xFFFFu) << 16);
-}
-
-__device__ __forceinline__ unsigned key_count(const unsigned* bins, int s, bool regular) {
-    if (!regular) return bins[s & (WINDOW - 1)];
-    if (s >= REGULAR_KEYS) return 0u;
-    const unsigned n = bins[s <= SPAN ? SPAN - s : NEGATIVE + s - SPAN];
-    return s == SPAN ? n + bins[NEGATIVE] : n;
+// irregular rows: position p of the whole key space (0 = the largest value) -> bf16 pattern
+__device__ __forceinline__ unsigned full_bits(int p) {
+    const unsigned k = 65535u - (unsigned)p;
+    return (k & 0x8000u) ? k ^ 0x8000u : ~k & 0xFFFFu;
 }
 
 // irregular rows: key of a bf16 pattern, -1 for an entry without weight (-inf, NaN); -0 counts as +0
@@ -182,6 +169,24 @@ __device__ __forceinline__ u32x4 row_chunk(const bf16_t* lc, const bf16_t* lu, i
     return t;
 }
 
+// One more in the bins of a word's two entries: bin = clamped magnitude, the sign bit in place (in `word`).  The addresses are
+// formed in three instructions by hand (merge the signs, shift either half), where the compiler takes five.
+__device__ __forceinline__ void count_two(unsigned* bins, unsigned word, unsigned clamped) {
+    unsigned at, lo, hi;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(at) : "v"(word), "s"(0x80008000u), "v"(clamped));
+    asm("v_lshlrev_b32_sdwa %0, %2, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:WORD_0" : "=v"(lo) : "v"(at), "v"(2u));
+    asm("v_lshlrev_b32_sdwa %0, %2, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:WORD_1" : "=v"(hi) : "v"(at), "v"(2u));
+    atomicAdd((unsigned*)((unsigned char*)bins + lo), 1u);
+    atomicAdd((unsigned*)((unsigned char*)bins + hi), 1u);
+}
+
+// 1 in each half that is zero, else 0 (by hand: the compiler turns the saturating 1 - x into compares and selects)
+__device__ __forceinline__ unsigned zero_halves(unsigned x) {
+    unsigned r;
+    asm("v_pk_sub_u16 %0, %1, %2 clamp" : "=v"(r) : "v"(0x00010001u), "v"(x));
+    return r;
+}
+
 // Draws the token of one row.  EPI: also leaves the row's confidence (rules of llada_remask_scores) in `conf`.
 template <bool EPI>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
@@ -198,7 +203,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         if (i < (SPAN + 2) / 4) ((u32x4*)(bins + NEGATIVE))[i] = (u32x4){0u, 0u, 0u, 0u};
     }
     if (tid < (SPAN + 2) % 4) bins[NEGATIVE + (SPAN + 2) / 4 * 4 + tid] = 0u;
-    if (tid < SLOTS) sh.slot_tot[tid] = 0u;
+    if (tid < SLOTS / 2) sh.slot_tot[tid] = 0u;
     if (tid == 0) sh.irregular = 0;
 
     __syncthreads();
@@ -224,15 +229,15 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     }
     if (lu) {
 #pragma unroll
-        for (int g = 0; g < SLOTS; g += 4) {
-            u32x4 b[4];
+        for (int g = 0; g < SLOTS; g += 8) {
+            u32x4 b[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 const int v0 = (tid + (g + i) * THREADS) * 8 - off;
                 if (v0 >= 0 && v0 + 8 <= V) b[i] = __builtin_nontemporal_load((const u32x4*)(lu + v0));
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 const int v0 = (tid + (g + i) * THREADS) * 8 - off;
                 if (v0 >= 0 && v0 + 8 <= V) q[g + i] = combine(q[g + i], b[i], a.cfg1);
             }
@@ -260,12 +265,11 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             const u16x2 mag = halves(q[i][e] & 0x7FFF7FFFu);
             const u16x2 idx = __builtin_elementwise_min(__builtin_elementwise_sub_sat(mag, (u16x2)((unsigned short)(MAG_LO - 1))),
                                                         (u16x2)((unsigned short)(SPAN + 1)));
-            const unsigned at = __builtin_bit_cast(unsigned, idx) | (q[i][e] & 0x80008000u);
-            atomicAdd(&bins[at & 0xFFFFu], 1u);
-            atomicAdd(&bins[at >> 16], 1u);
+            count_two(bins, q[i][e], __builtin_bit_cast(unsigned, idx));
         }
     }
     __syncthreads();
+    if (tid == 0) bins[0] += bins[NEGATIVE];     // zero of either sign (the test below holds before and after)
     // clamped bins that are not empty: zeros and -inf are as good as binned, anything else makes the row irregular
     if (bins[0] + bins[NEGATIVE] + bins[SPAN + 1] + bins[NEGATIVE + SPAN + 1] != 0u) {
         // smallest magnitude above zero, largest positive pattern, largest negative one but -inf
@@ -287,7 +291,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     }
     __syncthreads();
     const bool regular = sh.irregular == 0;
-    const double to_log2 = LOG2E / T;            // a distance from the largest logit -> log2 of its weight
+    // a distance from the largest logit -> log2 of its weight (temperature 0: all but the largest weigh nothing)
+    const double to_log2 = T > 0.0 ? fmin(LOG2E / T, 1.0e300) : 1.0e300;
 
     // An irregular row: counts one window of its keys into the bins, from memory again (such rows are rare and the
     // row's registers are better left alone).  All threads call it together.
@@ -307,54 +312,60 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         __syncthreads();
     };
 
-    // The row's values in order stand at positions 0 .. n_pos - 1: a regular row's occupied keys, gathered in a list; an
+    // The row's values in order stand at positions 0 .. n_pos - 1: a regular row's occupied ones, gathered in a list; an
     // irregular row's whole key space.  A chunk is 64 positions.
     float m = 0.f;                   // the largest value
     int n_pos = 65536;
-    auto key_at = [&](int p) { return regular ? (int)sh.keys[p] : p; };
-    // position p: its value minus the largest, the weight at that distance
-    auto distance = [&](int p) {
-        const float v = key_value(key_at(p), regular);
-        return v == m ? 0.0 : (double)v - (double)m;
+    struct Entries {
+        unsigned n;                  // of this position
+        float v;
+        double dl;                   // v minus the largest (0 where there is no entry)
     };
-    auto weight_at = [&](double dl) { return dl == 0.0 ? 1.0 : T > 0.0 ? exp2_neg(dl * to_log2) : 0.0; };
+    auto bits_at = [&](int p) { return regular ? (unsigned)sh.patterns[p] : full_bits(p); };
+    auto value_at = [&](int p) { return __uint_as_float(bits_at(p) << 16); };
+    auto entries_at = [&](int p) {
+        const int at = min(p, n_pos - 1);
+        const unsigned bits = bits_at(at), mag = bits & 0x7FFFu;
+        Entries x;
+        x.n = bins[regular ? (int)((mag < MAG_LO ? 0u : mag - (MAG_LO - 1u)) | (bits & 0x8000u)) : (at & (WINDOW - 1))];
+        if (p >= n_pos) x.n = 0u;
+        x.v = __uint_as_float(bits << 16);
+        const double dl = (double)x.v - (double)m;
+        x.dl = x.v == m || x.n == 0u ? 0.0 : dl;
+        return x;
+    };
     double s_sum = 0.0;              // epilogue: sum of exp(l - m) over the row
     auto total_chunk = [&](int c) {
-        const int p = c * 64 + lane;
-        unsigned n = 0;
-        double dl = 0.0;
-        if (p < n_pos) {
-            const int s = key_at(p);
-            n = key_count(bins, s, regular);
-            const float v = key_value(s, regular);
-            dl = v == m ? 0.0 : (double)v - (double)m;
-            if (EPI && n) s_sum += seen(n, v) * exp2_neg(dl * LOG2E);
-        }
-        const double ms = wave_scan(n ? n * weight_at(dl) : 0.0);
-        const unsigned cs = wave_scan(n);
+        const Entries x = entries_at(c * 64 + lane);
+        const double ms = wave_scan(x.n * exp2_neg(x.dl * to_log2));
+        const unsigned cs = wave_scan(x.n);
         if (lane == 63) {
             sh.cnt[c] = cs;
             sh.mass[c] = ms;
         }
+        if (EPI && x.n) s_sum += seen(x.n, x.v) * exp2_neg(x.dl * LOG2E);
     };
 
     // ---- totals of the chunks: entries, weight ----
     if (regular) {
-        // group i * 16 + wave of 64 keys: neighbouring groups, which are full together, are spread over the waves
+        // group g = i * 16 + wave of 64 keys: neighbouring groups, which are full together, are spread over the waves.  A
+        // group's keys have one sign; group SPAN / 64 starts with zero, the last group has one key.  (Few instructions a
+        // group: every wave looks through 16 of them.)
+        static_assert(SPAN % 64 == 0 && REGULAR_KEYS % 64 == 1, "groups");
         unsigned n[PER_WAVE];
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
-            const int s = (i * NWV + wave) * 64 + lane;
-            n[i] = bins[s <= SPAN ? SPAN - s : NEGATIVE + min(s - SPAN, SPAN + 1)];
-            if (i == SPAN / 64 / NWV && s == SPAN) n[i] += bins[NEGATIVE];          // zero of either sign
-            if (i == PER_WAVE - 1 && s >= REGULAR_KEYS) n[i] = 0u;
+            const int g = i * NWV + wave;                    // (uniform)
+            const unsigned* at = bins + (g < SPAN / 64 ? SPAN - g * 64 : NEGATIVE + min(g * 64 - SPAN, SPAN - 63));
+            n[i] = at[g < SPAN / 64 ? -lane : lane];
+            if (i == PER_WAVE - 1) n[i] = g > REGULAR_KEYS / 64 ? 0u : g == REGULAR_KEYS / 64 ? (lane == 63 ? n[i] : 0u) : n[i];
         }
-        uint64_t any[PER_WAVE];
+        if (wave == SPAN / 64 % NWV && lane == 0) n[SPAN / 64 / NWV] = bins[0];
         unsigned held = 0;
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
-            any[i] = __builtin_amdgcn_ballot_w64(n[i] != 0u);
-            if (lane == i) held = (unsigned)__popcll(any[i]);
+            const unsigned c = (unsigned)__popcll(__builtin_amdgcn_ballot_w64(n[i] != 0u));
+            if (lane == i) held = c;
         }
         if (lane < PER_WAVE) sh.cnt[lane * NWV + wave] = held;
         __syncthreads();
@@ -367,11 +378,16 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         base += (j > 0 ? g[0] : 0u) + (j > 1 ? g[1] : 0u) + (j > 2 ? g[2] : 0u);
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
-            const unsigned before = __builtin_amdgcn_mbcnt_hi((unsigned)(any[i] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)any[i], 0u));
-            if (n[i]) sh.keys[from_lane(base, 4 * i + (wave >> 2)) + before] = (unsigned short)((i * NWV + wave) * 64 + lane);
+            const uint64_t any = __builtin_amdgcn_ballot_w64(n[i] != 0u);
+            if (any == 0) continue;
+            const unsigned before = __builtin_amdgcn_mbcnt_hi((unsigned)(any >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)any, 0u));
+            const int g = i * NWV + wave;
+            const unsigned bits = g < SPAN / 64 ? MAG_HI - 1u - g * 64 - lane : g == REGULAR_KEYS / 64 ? 0x8000u + MAG_HI - 1u
+                                                                                                  : 0x8000u + MAG_LO - 1u + (g * 64 - SPAN) + lane;
+            if (n[i]) sh.patterns[from_lane(base, 4 * i + (wave >> 2)) + before] = (unsigned short)(bits == 0x8000u + MAG_LO - 1u ? 0u : bits);
         }
         __syncthreads();
-        if (n_pos > 0) m = key_value(sh.keys[0], true);
+        if (n_pos > 0) m = value_at(0);
 #pragma unroll 1
         for (int c = wave; c * 64 < n_pos; c += NWV) total_chunk(c);
     } else {
@@ -382,7 +398,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             if (!found) {
                 int mine = 0x7fffffff;
                 for (int c = c_lo + wave; c < c_hi; c += NWV) {
-                    const uint64_t any = __builtin_amdgcn_ballot_w64(key_count(bins, c * 64 + lane, false) != 0u);
+                    const uint64_t any = __builtin_amdgcn_ballot_w64(bins[(c * 64 + lane) & (WINDOW - 1)] != 0u);
                     if (any != 0 && mine == 0x7fffffff) mine = c * 64 + __builtin_ctzll(any);
                 }
                 if (lane == 0) sh.first[wave] = mine;
@@ -391,7 +407,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
 #pragma unroll
                 for (int w = 0; w < NWV; ++w) top = min(top, sh.first[w]);
                 found = top != 0x7fffffff;
-                if (found) m = key_value(top, false);
+                if (found) m = value_at(top);
                 __syncthreads();
             }
             for (int c = c_lo + wave; c < c_hi; c += NWV) total_chunk(c);
@@ -480,11 +496,11 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     };
     auto look_inside = [&](int c) {
         if (!regular) count_window(c / (WINDOW / 64));
+        const Entries e = entries_at(c * 64 + lane);
         Inside x;
-        const int p = c * 64 + lane;
-        x.n = p < n_pos ? key_count(bins, key_at(p), regular) : 0u;
-        x.w = x.n ? weight_at(distance(p)) : 0.0;
-        x.before = sh.mass[c] + lane_before(wave_scan(x.n ? x.n * x.w : 0.0));
+        x.n = e.n;
+        x.w = exp2_neg(e.dl * to_log2);
+        x.before = sh.mass[c] + lane_before(wave_scan(x.n * x.w));
         x.upto = sh.cnt[c] + wave_scan(x.n);
         return x;
     };
@@ -528,10 +544,11 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             // the first position whose weight is below min_p: weights fall along the positions, 64 probes a round.  Compared before the
             // exponential: min_p = 1 keeps exactly the entries that equal the largest, whatever T.
             const double edge = T * log(min_p);
+            auto below = [&](int p) { return value_at(p) == m ? 0.0 : (double)value_at(p) - (double)m; };
             int cut = 0, hi = n_pos;
             while (cut < hi) {
                 const int step = (hi - cut + 63) / 64, s = cut + (lane + 1) * step - 1;
-                const uint64_t fails = __builtin_amdgcn_ballot_w64(s >= hi || distance(s) < edge);
+                const uint64_t fails = __builtin_amdgcn_ballot_w64(s >= hi || below(s) < edge);
                 const int f = fails ? __builtin_ctzll(fails) : 64;
                 hi = min(hi, cut + (f + 1) * step - 1);
                 cut = cut + f * step;
@@ -569,7 +586,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         if (wave == 0 && lane == at) {
             sh.j = (int)(rank - (y.upto - y.n) - 1u);
             sh.tied = (int)y.n;
-            sh.value = key_value(key_at(c * 64 + lane), regular);
+            sh.value = value_at(c * 64 + lane);
             sh.prob = (float)(y.w / total);
         }
     }
@@ -581,50 +598,48 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     const unsigned pat = bits * 0x00010001u;
     const unsigned msk = bits == 0u ? 0x7FFF7FFFu : 0xFFFFFFFFu;      // zero: either sign
     const bool single = sh.tied == 1;            // (uniform)
-    unsigned hits = 0;                           // chunks of this lane with a match
-    auto nearest = [&](int i) {                  // zero in a half: a match in that half of some word of chunk i
-        u16x2 x[4];
+    int slot = -1;                               // the chunk that holds the entry, in the lane that holds it
+    unsigned skip = 0;                           // matches of that chunk before the entry
+    auto differs = [&](int i, int e) { return (q[i][e] ^ pat) & msk; };       // zero in a half: a match
+    if (single) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = halves((q[i][e] ^ pat) & msk);
-        return __builtin_elementwise_min(__builtin_elementwise_min(x[0], x[1]), __builtin_elementwise_min(x[2], x[3]));
-    };
-    auto zero_half = [](u16x2 v) {
-        const unsigned b = __builtin_bit_cast(unsigned, v);
-        return ((b & 0xFFFFu) == 0u) | (b < 0x10000u);
-    };
+        for (int g = 0; g < SLOTS; g += 4) {     // most waves hold no match: four chunks are ruled out at a time
+            u16x2 least = halves(differs(g, 0));
 #pragma unroll
-    for (int g = 0; g < SLOTS; g += 4) {         // most waves hold no match: four chunks are ruled out at a time
-        u16x2 x[4];
+            for (int i = 1; i < 16; ++i) least = __builtin_elementwise_min(least, halves(differs(g + i / 4, i & 3)));
+            if (__builtin_amdgcn_ballot_w64(zero_halves(__builtin_bit_cast(unsigned, least)) != 0u) == 0) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = nearest(g + i);
-        if (__builtin_amdgcn_ballot_w64(zero_half(__builtin_elementwise_min(__builtin_elementwise_min(x[0], x[1]), __builtin_elementwise_min(x[2], x[3])))) == 0) continue;
+            for (int i = g; i < g + 4; ++i) {
+                u16x2 x = halves(differs(i, 0));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) hits |= (unsigned)zero_half(x[i]) << (g + i);
-    }
-    int slot = single && hits ? __builtin_ctz(hits) : -1;     // the chunk that holds the entry, in the lane that holds it
-    unsigned skip = 0;                                        // matches of that chunk before the entry
-    if (!single) {
-        unsigned mine[SLOTS / 4] = {};           // matches of each chunk, a byte each
-        const u16x2 one = {1, 1};
+                for (int e = 1; e < 4; ++e) x = __builtin_elementwise_min(x, halves(differs(i, e)));
+                if (zero_halves(__builtin_bit_cast(unsigned, x)) != 0u) slot = i;
+            }
+        }
+    } else {
+        unsigned mine[SLOTS / 2];                // matches of each chunk, 16 bits each (a slot's row-wide total fits as well)
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-            if (__builtin_amdgcn_ballot_w64((hits >> i) & 1u) == 0) continue;
-            u16x2 miss = {0, 0};
+        for (int i = 0; i < SLOTS; i += 2) {
+            unsigned n[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) miss += __builtin_elementwise_min(halves((q[i][e] ^ pat) & msk), one);
-            const unsigned n = 8u - (unsigned)(miss[0] + miss[1]);
-            mine[i >> 2] |= n << (8 * (i & 3));
-            const unsigned sum = wave_scan(n);
-            if (lane == 63) atomicAdd(&sh.slot_tot[i], sum);
+            for (int k = 0; k < 2; ++k) {
+                // sums of the packed halves: at most 4 a half
+                const unsigned h = zero_halves(differs(i + k, 0)) + zero_halves(differs(i + k, 1)) + zero_halves(differs(i + k, 2)) +
+                                   zero_halves(differs(i + k, 3));
+                n[k] = (h & 0xFFFFu) + (h >> 16);
+            }
+            mine[i / 2] = n[0] | n[1] << 16;
+            const unsigned sum = wave_scan(mine[i / 2]);
+            if (lane == 63 && sum) atomicAdd(&sh.slot_tot[i / 2], sum);
         }
         __syncthreads();
-        const unsigned upto = wave_scan(lane < SLOTS ? sh.slot_tot[lane & (SLOTS - 1)] : 0u);
+        const unsigned upto = wave_scan(lane < SLOTS ? (sh.slot_tot[(lane & (SLOTS - 1)) / 2] >> (16 * (lane & 1))) & 0xFFFFu : 0u);
         const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > (unsigned)sh.j));
         const unsigned left = (unsigned)sh.j - from_lane(lane_before(upto), at);
         unsigned n_here = 0;
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i)
-            if (i == at) n_here = (mine[i >> 2] >> (8 * (i & 3))) & 255u;
+            if (i == at) n_here = (mine[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
         const unsigned incl = wave_scan(n_here);
         if (lane == 63) sh.wave_tot[wave] = incl;
         __syncthreads();
@@ -679,11 +694,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
                 const int p_lo = regular ? 0 : win * WINDOW, p_hi = regular ? n_pos : p_lo + WINDOW;
 #pragma unroll 1
                 for (int p = p_lo + tid; p < p_hi; p += THREADS) {
-                    const int s = key_at(p);
-                    const unsigned n = key_count(bins, s, regular);
-                    if (n == 0u) continue;
-                    const float v = key_value(s, regular);
-                    es += seen(n, v) * term(v == m ? 0.0 : (double)v - (double)m);
+                    const Entries x = entries_at(p);
+                    if (x.n) es += seen(x.n, x.v) * term(x.dl);
                 }
             }
             es = wave_total(es);
