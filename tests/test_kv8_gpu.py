@@ -335,3 +335,73 @@ def test_every_way_to_deal_the_work(lib, nq, splits, n_q, start, fresh):
         check_attend(make(n, L, H, "e4m3"), rows(L + nq, n, L, H), H, n_q, "e4m3", left_mask(n, L, n_q), fresh, start)
     finally:
         lib.llada_attn_kv8_force(0, 0)
+
+
+@pytest.mark.parametrize("n_q,b_len,start", [(1, 200, 37), (20, 330, 64), (40, 130, 270), (140, 1, 399), (140, 400, 0), (5, 64, 128)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_block_of_another_length_than_the_queries(lib, n_q, b_len, start, masked):
+    """Fresh rows for more or fewer tokens than there are queries: several fresh tiles for few queries, one row for many."""
+    n, L, H, dtype = 2, 400, 2, "e4m3"
+    m = left_mask(n, L, b_len) if masked else None
+    if masked:
+        m[1, start:start + b_len:3] = 0
+    mt = None if m is None else torch.from_numpy(m).cuda()
+    x, y, f = rows(50, n, L, H), rows(51, n, n_q, H), rows(52, n, b_len, H)
+    c = make(n, L, H, dtype)
+    c.fill(0, x, mt)
+    out = c.attend(0, y, mt, block=f, block_start=start)
+    _, k, v = split(x, H)
+    k, v = okv.held(k, dtype, m), okv.held(v, dtype, m)
+    q = split(y, H)[0]
+    _, k[:, start:start + b_len], v[:, start:start + b_len] = split(f, H)
+    want, spread = okv.attend(q, k, v, m)
+    got = out.double().cpu().numpy().reshape(n, n_q, H, 128)
+    e = 130 * 2.0 ** -24 * np.sqrt((q ** 2).sum(-1)).max() * np.sqrt((k ** 2).sum(-1)).max() / np.sqrt(128) + 2.0 ** -19
+    assert (np.abs(got - want) <= 2.0 ** -8 * (spread + np.abs(want)) + (2 * e + 2.0 ** -20) * spread).all()
+
+
+def test_offsets_past_32_bits(lib):
+    """A cache of more than 4 GiB: the last sequence's results and values equal those of a cache of that sequence alone."""
+    n, L, H, n_q = 5, 131072, 32, 3
+    new, q = rows(60, n, 130, H), rows(61, n, n_q, H)
+    big, one = make(n, L, H, "e4m3"), make(1, L, H, "e4m3")
+    assert big.layer_bytes > 2 ** 32
+    try:
+        lib.llada_attn_kv8_force(1, 1)
+        for c, sel in ((big, slice(None)), (one, slice(n - 1, n))):
+            c.update(0, new[sel], L - 130)
+            c.update(0, new[sel, :64], 64)
+        a, b = big.attend(0, q, block=new, block_start=L - 200), one.attend(0, q[n - 1:], block=new[n - 1:], block_start=L - 200)
+    finally:
+        lib.llada_attn_kv8_force(0, 0)
+    assert torch.equal(a[n - 1:], b) and b.abs().max() > 0
+    kb, ko = big.read(0)[0], one.read(0)[0]
+    assert torch.equal(kb[n - 1], ko[0]) and ko[0, -100:].abs().max() > 0
+    assert torch.equal(kb[0, 64:128], okv_held_like(new[0, :64], H))
+
+
+def okv_held_like(rows_, H):
+    k = rows_.double().cpu().numpy().reshape(1, 64, 3, H, 128)[:, :, 1]
+    return torch.from_numpy(okv.held(k, "e4m3")[0]).cuda().to(torch.bfloat16)
+
+
+def test_two_streams_at_once(lib):
+    """Calls on two caches from two streams, key splits' scratch in use, give what they give one after the other."""
+    L, H, n_q = 4096, 32, 16
+    cs = [make(1, L, H, "e4m3") for _ in range(2)]
+    qs = [rows(70 + i, 1, n_q, H) for i in range(2)]
+    for i, c in enumerate(cs):
+        c.fill(0, rows(72 + i, 1, L, H))
+    want = [c.attend(0, q) for c, q in zip(cs, qs)]
+    assert lib.llada_attn_kv8_workspace_bytes(1, n_q, L, H) > 0
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(cs[i].attend(0, qs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for t in got[i]:
+            assert torch.equal(t, want[i])

@@ -225,3 +225,40 @@ def test_replayed_graph(lib):
         want = sample_tokens(x, 0.8, top_p=0.9, uniforms=u)
         torch.cuda.synchronize()
         assert torch.equal(tok, want)
+
+
+def test_offsets_past_32_bits(lib):
+    """More than 2^31 logits: the last rows' tokens are those of a call on them alone."""
+    from llada_amd import sample_tokens
+    n, V = 17100, 126464
+    x = torch.zeros((n, V), dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2 ** 31
+    x[-5:] = logits(90, 5, V)
+    x[7] = x[-1]
+    u = torch.rand(n, dtype=torch.float64, device="cuda")
+    tok = sample_tokens(x, 0.9, top_p=0.95, uniforms=u)
+    assert torch.equal(tok[-5:], sample_tokens(x[-5:].clone(), 0.9, top_p=0.95, uniforms=u[-5:]))
+    keep = int(np.ceil(0.95 * V))                       # a row of zeros: the u-th of its first 95 %, in index order
+    assert torch.equal(tok[100:-5], (u[100:-5] * keep).to(torch.int64))
+
+
+def test_uniforms_outside_their_range_stay_inside_the_row(lib):
+    from llada_amd import sample_tokens
+    x = logits(91, 6, 700)
+    u = torch.tensor([-1.0, 1.0, 2.0, float("nan"), float("inf"), -float("inf")], dtype=torch.float64, device="cuda")
+    for kw in (dict(), dict(top_k=5), dict(top_p=0.5), dict(min_p=0.3), dict(temperature=0.0)):
+        t = sample_tokens(x, uniforms=u, **kw)
+        assert ((t >= 0) & (t < 700)).all()
+
+
+def test_parameter_arrays_outside_their_ranges_act_like_the_nearest_end(lib):
+    from llada_amd import sample_tokens
+    x, u = logits(92, 4, 900), torch.from_numpy(uniforms(92, 4)).cuda()
+    base = sample_tokens(x, uniforms=u)
+    dev = dict(device="cuda")
+    assert torch.equal(base, sample_tokens(x, uniforms=u, top_p=torch.tensor([1.5, 2.0, float("nan"), 1.0], **dev)))
+    assert torch.equal(base, sample_tokens(x, uniforms=u, top_k=torch.tensor([0, -5, -1, 2 ** 31 - 1], **dev)))
+    assert torch.equal(base, sample_tokens(x, uniforms=u, min_p=torch.tensor([0.0, -1.0, float("nan"), -0.5], **dev)))
+    first = x.float().argmax(dim=1)
+    for k in (dict(top_p=torch.full((4,), -0.5, **dev)), dict(min_p=torch.full((4,), 7.0, **dev)), dict(temperature=torch.tensor([0.0, -1.0, float("nan"), 0.0], **dev))):
+        assert torch.equal(first, sample_tokens(x, uniforms=u, **k))
