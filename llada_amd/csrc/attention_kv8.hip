@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
     const int n_fresh = a.n_units - a.n_cached;
     const int u_begin = ks * a.per_split, u_end = min(a.n_units, u_begin + a.per_split);
     const int c_begin = max(u_begin, n_fresh);
-    int u = c_begin + ((kg - (c_begin - u_begin)) & (NK - 1));          // this wave's first cached one
+    const bool idle = q0 >= a.n_q;                                      // (a wave behind the last query only helps to fetch)
+    int u = idle ? u_end : c_begin + ((kg - (c_begin - u_begin)) & (NK - 1));           // this wave's first cached one
 
     // The first cached tile's keys are fetched ahead of everything else.
     auto tile_of = [&](int i) { i -= n_fresh; return i < a.skip_from ? i : i + a.skipped; };
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
     float ks_next = 1.f, vs_next = 1.f;
     if (u < u_end) {
         t = tile_of(u);
-        load_keys(t);
+        if constexpr (NK > 1) load_keys(t);
         mb = mask_byte(t);
         ks_next = scales[2 * t];
         vs_next = scales[2 * t + 1];
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
         const int f = NK == 1 ? f_next : f_next + ((kg + u_begin - f_next) & (NK - 1));     // the tile of this round that is this wave's
         const int f0 = f * KV8_TOKENS;
         if (NK == 1 && f + 1 < f_end) fetch_fresh(f + 1, buf ^ 1);      // (the buffer of the last round is no longer read)
-        if (f < min(f_next + AHEAD, f_end)) {
+        if (!idle && f < min(f_next + AHEAD, f_end)) {
             unsigned char* const k_lds = lds + (NK == 1 ? buf : f - f_next) * FRESH;
             unsigned char* const v_lds = k_lds + KV8_TOKENS * 256;
             const int fk = f0 + lane;
@@ -259,33 +260,54 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
                 for (int i = 0; i < KV8_TOKENS / 4; ++i)
                     if (!(((unmasked & there) >> (i * 4 + (lane >> 4))) & 1)) *(u32x4*)(v_lds + i * 1024 + lane * 16) = (u32x4){0u, 0u, 0u, 0u};
             }
+            // One key group: reads go out four products ahead (left to itself, the compiler saves registers and waits out each
+            // read alone); several: their registers hold the first cached tile's keys.
+            auto hold = [] { if constexpr (NK == 1) __builtin_amdgcn_sched_barrier(0); };
             f32x16 s[2];
+            bf16x8 kf[2][4];
+            auto read_keys = [&](int g) {                               // of products 4 g .. + 3: keys 32 (g >> 1) .., dims 32 (g & 1) .. of each half
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+                for (int i = 0; i < 4; ++i)
+                    kf[g & 1][i] = *(const bf16x8*)(k_lds + ((g >> 1) * 32 + r) * 256 + (((8 * hg + 4 * (g & 1) + i) ^ (r & 15)) * 16));
+            };
+            read_keys(0);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+            for (int g = 0; g < 4; ++g) {
+                if (g < 3) read_keys(g + 1);
+                hold();
+                if ((g & 1) == 0) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bf16x8 kf = *(const bf16x8*)(k_lds + (kb * 32 + r) * 256 + (((8 * hg + i) ^ (r & 15)) * 16));
-                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i], s[kb], 0, 0, 0);
+                    for (int e = 0; e < 16; ++e) s[g >> 1][e] = 0.f;
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[g >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[g & 1][i], qf[4 * (g & 1) + i], s[g >> 1], 0, 0, 0);
+                hold();
             }
             bf16x8 pb[2][2];
             softmax_tile(s, unmasked & there, a.scale_log2e, 0.f, 1.f, w, pb, hg);
             const int q4 = (lane & 15) >> 2, p4 = lane & 3, g1 = (lane >> 4) & 1;
             const unsigned char* const vrow = v_lds + (4 * hg + q4) * 256 + 32 * g1 + 8 * p4;
+            s16x4 vf[2][4][2];
+            auto read_values = [&](int g) {                             // of keys 16 g .. + 15
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+                for (int db = 0; db < 4; ++db) {
+                    const unsigned char* p = vrow + g * 16 * 256 + ((db * 64) ^ (q4 * 64));
+                    vf[g & 1][db][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p);
+                    vf[g & 1][db][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 8 * 256));
+                }
+            };
+            read_values(0);
 #pragma unroll
-                for (int ss = 0; ss < 2; ++ss)
+            for (int g = 0; g < 4; ++g) {
+                if (g < 3) read_values(g + 1);
+                hold();
 #pragma unroll
-                    for (int db = 0; db < 4; ++db) {
-                        const unsigned char* p = vrow + (kb * 32 + 16 * ss) * 256 + ((db * 64) ^ (q4 * 64));
-                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p);
-                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 8 * 256));
-                        const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                        w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pb[kb][ss], w.o[db], 0, 0, 0);
-                    }
+                for (int db = 0; db < 4; ++db) {
+                    const s16x8 v = __builtin_shufflevector(vf[g & 1][db][0], vf[g & 1][db][1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pb[g >> 1][g & 1], w.o[db], 0, 0, 0);
+                }
+                hold();
+            }
         }
         if constexpr (NK == 1) {
             buf ^= 1;
@@ -297,7 +319,10 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
         }
     }
     // ---- cached tiles ----
-    if (u < u_end) load_values(t);
+    if (u < u_end) {
+        if constexpr (NK == 1) load_keys(t);
+        load_values(t);
+    }
     for (; u < u_end; u += NK) {
         const uint64_t valid = live_keys(t, mb);
         const float kscale = ks_next, vscale = vs_next;
