@@ -15,9 +15,17 @@ def truncates(temperature, top_k, top_p, min_p):
     return temperature != 0 and (top_k > 0 or top_p < 1.0 or min_p > 0.0)
 
 
+TOP_K_MAX = 2 ** 31 - 1
+
+
+def _top_k(k):
+    """A top_k for the library's 32 bits: any larger one keeps the whole row as well (a negative one is refused there)."""
+    return k.clamp(-1, TOP_K_MAX) if isinstance(k, torch.Tensor) else max(-1, min(int(k), TOP_K_MAX))
+
+
 def scalar_sampling(temperature, top_k, top_p, min_p, uniforms=None):
     """The C parameters for one value of each; ``uniforms``: float64 tensor, or None for the library's own stream."""
-    return _lib.Sampling(float(temperature), float(top_p), float(min_p), int(top_k), None, None, None, None, _lib.ptr(uniforms))
+    return _lib.Sampling(float(temperature), float(top_p), float(min_p), _top_k(top_k), None, None, None, None, _lib.ptr(uniforms))
 
 
 def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uniforms=None, uncond_logits=None, cfg_scale=0.0,
@@ -28,7 +36,7 @@ def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uni
     float64: top-k keeps the first ``top_k`` (0: all), top-p the shortest prefix of those with at least ``top_p`` of
     their mass, min-p the entries with w_i >= ``min_p``; what all three keep (at least one entry) is sampled: the token is
     the first whose running mass exceeds u times the kept total.  temperature 0 gives the arg-max.  ``temperature``,
-    ``top_k``, ``top_p`` and ``min_p`` may each be a tensor with one value per row.
+    ``top_k``, ``top_p`` and ``min_p`` may each be a tensor with one value per row (held in float32 and int32).
 
     ``uniforms`` [...] float64 in [0, 1); without it u comes from the library's Philox stream, counters (row, step) with
     the rows numbered from ``row_offset``.  ``uncond_logits`` (same shape): combined with ``cfg_scale`` first, as
@@ -50,7 +58,7 @@ def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uni
         if un.stride() != rows.stride() or (un.data_ptr() - rows.data_ptr()) % 16:
             rows, un, stride = rows.clone(memory_format=torch.contiguous_format), un.clone(memory_format=torch.contiguous_format), vocab
     arrays, keep = [None] * 4, []
-    scalars = [temperature, top_k, top_p, min_p]
+    scalars = [temperature, _top_k(top_k), top_p, min_p]
     for i, (v, dtype, off) in enumerate(zip(scalars, (torch.float32, torch.int32, torch.float32, torch.float32), (1.0, 0, 1.0, 0.0))):
         if isinstance(v, torch.Tensor):
             if v.dim() and v.shape != lead:
@@ -67,7 +75,7 @@ def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uni
         tokens = torch.empty(lead, dtype=torch.int64, device=dev)
         probs = torch.empty(lead, dtype=torch.float32, device=dev) if return_probs else None
         if n:
-            s = _lib.Sampling(float(t), float(p), float(q), int(k), *arrays, _lib.ptr(u))
+            s = _lib.Sampling(float(t), float(p), float(q), k, *arrays, _lib.ptr(u))
             _lib.check(lib.llada_sample_rows(rows.data_ptr(), _lib.ptr(un), stride, float(cfg_scale), n, vocab, C.byref(s), seed, step,
                                              row_offset, tokens.data_ptr(), _lib.ptr(probs), _lib.stream_ptr(dev.index)))
     return (tokens, probs) if return_probs else tokens

@@ -262,3 +262,13 @@ def test_parameter_arrays_outside_their_ranges_act_like_the_nearest_end(lib):
     first = x.float().argmax(dim=1)
     for k in (dict(top_p=torch.full((4,), -0.5, **dev)), dict(min_p=torch.full((4,), 7.0, **dev)), dict(temperature=torch.tensor([0.0, -1.0, float("nan"), 0.0], **dev))):
         assert torch.equal(first, sample_tokens(x, uniforms=u, **k))
+
+
+def test_top_k_past_32_bits_keeps_the_row(lib):
+    from llada_amd import sample_tokens
+    x, u = logits(90, 6, 1000), torch.from_numpy(uniforms(90, 6)).cuda()
+    want = sample_tokens(x, uniforms=u)
+    assert torch.equal(sample_tokens(x, top_k=2 ** 32 + 1, uniforms=u), want)
+    assert torch.equal(sample_tokens(x, top_k=torch.full((6,), 2 ** 32 + 1, device="cuda"), uniforms=u), want)
+    with pytest.raises(AssertionError):
+        sample_tokens(x, top_k=5 - 2 ** 32, uniforms=u)
