@@ -15,7 +15,7 @@
 // probabilities (p 2^e = 2^(s - m + e)), so neither costs an instruction per element.
 //
 // Scores, running maximum, sums and outputs are float32; P is rounded to bf16 once for the matrix unit, like the keys' and
-// values' bf16 forms it multiplies (relative 2^-9 per term, averaged over the terms).
+// values' bf16 forms it multiplies (at most 2^-8 of a term, averaged over the terms).
 #include "kv8.h"
 
 namespace {

@@ -12,6 +12,12 @@ from . import _lib
 HEAD_DIM = 128
 
 
+def _overlap(a, b):
+    """Whether the memory two tensors span has bytes in common."""
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 class KVCache8:
     """Keys and values of ``n_layers`` layers, ``n_seq`` sequences of ``seq_len`` tokens and ``n_heads`` heads of 128.
 
@@ -23,6 +29,8 @@ class KVCache8:
             raise NotImplementedError(f"kv cache dtype {dtype!r} (one of {sorted(_lib.KV_TYPES)})")
         if min(n_seq, seq_len, n_heads, n_layers) < 1:
             raise ValueError("a cache needs at least one sequence, token, head and layer")
+        if torch.device(device).type != "cuda":
+            raise ValueError(f"a KVCache8 lives in GPU memory, not on {device}")
         self.lib = _lib.load()
         self.n_seq, self.seq_len, self.n_heads, self.n_layers, self.dtype = n_seq, seq_len, n_heads, n_layers, dtype
         self.d = n_heads * HEAD_DIM
@@ -113,7 +121,8 @@ class KVCache8:
         """softmax(q k^T / sqrt(128)) v of ``q`` [n_seq, n_q, >= d] (bf16 rows, head h at columns h * 128) over every
         unmasked token, no causal mask -> [n_seq, n_q, d] bf16.  ``block`` [n_seq, len, >= 3 d]: fresh [Q | K | V] rows
         whose keys and values stand in for the cached tokens from ``block_start`` on (the cache is only read); in a
-        cached denoise step q and block are the same rows.  A sequence without an unmasked token gives zeros."""
+        cached denoise step q and block are the same rows.  A sequence without an unmasked token gives zeros.  ``out`` may be
+        q's own memory, not the block's."""
         at = self._layer(layer)
         if q.dim() != 3 or q.shape[1] < 1:
             raise ValueError(f"q: [{self.n_seq}, n_q, >= {self.d}] is wanted, not {list(q.shape)}")
@@ -133,6 +142,8 @@ class KVCache8:
                 out = torch.empty((self.n_seq, n_q, self.d), dtype=torch.bfloat16, device=self.device)
             elif tuple(out.shape) != (self.n_seq, n_q, self.d) or out.dtype != torch.bfloat16 or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16:
                 raise ValueError(f"out: a contiguous bfloat16 [{self.n_seq}, {n_q}, {self.d}] on {self.device} is wanted")
+            elif bx is not None and _overlap(out, bx):
+                raise ValueError("out overlaps the block's rows, which every head's queries read")
             need = self._ws_bytes.get(n_q)
             if need is None:
                 need = self._ws_bytes[n_q] = self.lib.llada_attn_kv8_workspace_bytes(self.n_seq, n_q, self.seq_len, self.n_heads)

@@ -99,3 +99,9 @@ def test_oracle_matches_torch_float8_cast():
             k = np.ceil(np.log2(np.abs(part).max() / 448.0))
             want = torch.from_numpy((part / 2.0 ** k).astype(np.float32)).to(torch.float8_e4m3fn).float().numpy().astype(np.float64) * 2.0 ** k
             assert np.array_equal(got[0, t:t + 64, h], want)
+
+
+def test_a_cache_needs_a_gpu():
+    from llada_amd import KVCache8
+    with pytest.raises(ValueError, match="GPU memory"):
+        KVCache8(1, 64, 2, device="cpu")

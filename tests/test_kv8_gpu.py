@@ -405,3 +405,19 @@ def test_two_streams_at_once(lib):
     for i in range(2):
         for t in got[i]:
             assert torch.equal(t, want[i])
+
+
+@pytest.mark.parametrize("n,L,n_q", [(2, 200, 40), (1, 4200, 16), (2, 300, 150)])
+def test_output_in_the_queries_memory_but_not_in_the_blocks(lib, n, L, n_q):
+    from llada_amd import KVCache8
+    H = 4
+    cache = KVCache8(n, L, H)
+    cache.fill(0, torch.randn(n, L, 3 * H * 128, device="cuda").to(torch.bfloat16))
+    q = torch.randn(n, n_q, H * 128, device="cuda").to(torch.bfloat16)
+    want = cache.attend(0, q)
+    got = cache.attend(0, q, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+    block = torch.randn(n, n_q, 3 * H * 128, device="cuda").to(torch.bfloat16)
+    inside = block.view(-1)[: n * n_q * H * 128].view(n, n_q, H * 128)
+    with pytest.raises(ValueError, match="overlaps"):
+        cache.attend(0, block, block=block, out=inside)
