@@ -372,9 +372,9 @@ typedef struct llada_sampling {
 } llada_sampling;
 
 /* tokens[r] (int64) and, unless NULL, probs[r] (float32: the token's probability among the kept entries) for each row
- * of logits [n_rows, vocab] bf16, rows row_stride elements apart (uncond_logits likewise, at
- * the same offset from a 16-byte boundary, or NULL: combined with cfg_scale as llada_remask_scores does).  Parameter arrays and uniforms: [n_rows].  vocab <= 131072 (131065 where rows
- * are not 16-byte aligned).  Philox counters: (0, 0, row_offset + r, step). */
+ * of logits [n_rows, vocab] bf16, rows row_stride elements apart; uncond_logits likewise, at the same offset from a
+ * 16-byte boundary, or NULL: combined with cfg_scale as llada_remask_scores does.  Parameter arrays and uniforms:
+ * [n_rows].  vocab <= 131072 (131065 where rows are not 16-byte aligned).  Philox counters: (0, 0, row_offset + r, step). */
 int llada_sample_rows(const void* logits, const void* uncond_logits, int64_t row_stride, double cfg_scale, int32_t n_rows,
                       int32_t vocab, const llada_sampling* sampling, uint64_t seed, uint32_t step, uint32_t row_offset,
                       int64_t* tokens, float* probs, void* stream);
