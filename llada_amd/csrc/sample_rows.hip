@@ -11,41 +11,28 @@
 // alone (equal values are consecutive, in index order).  So nothing is sorted: a row's values are counted in LDS (one
 // integer atomic per entry: exact, order-free), exponentials in float64 are taken per distinct value, 64-value chunks of
 // the histogram are summed by waves in a fixed order, and the cuts and the token are found by prefix search over chunk
-// totals and then inside one chunk.  The row is read once and stays in registers (16 x 16 bytes a lane, 1024 lanes) for
-// the last step, which turns "the j-th entry of value v" into an index.
+// totals and then inside one chunk.  The row, or half of it, stays in registers (16 x 16 bytes a lane) for the last step,
+// which turns "the j-th entry of value v" into an index.
 //
-// The histogram has a bin for every bf16 value of magnitude in [2^-55, 2^8) of either sign and one for zero (2 x 32 KiB).
-// A row with another finite magnitude, an infinity of positive sign or a NaN is "irregular" (its clamped bins say so, at
-// no cost to other rows) and is counted over the whole 16-bit key space in four windows instead; -inf entries, NaNs
+// The histogram has a bin for every bf16 value of magnitude in [2^-55, 2^8), or [2^-35, 2^8), of either sign and one for
+// zero.  A row with another finite magnitude, an infinity of positive sign or a NaN is "irregular" (its clamped bins say
+// so, at no cost to other rows) and is counted over the whole 16-bit key space in windows instead; -inf entries, NaNs
 // included, have no weight and are never drawn.  A row with nothing else gives token 0 with probability 0.
 //
-// Bound by a CU's own work on a row, 49 to 55 thousand cycles: the histogram 18 to 28 (its LDS atomics alone 16: 64 random
-// bins meet in the banks, 8 cycles an instruction), listing the occupied bins 6, their weights 4, the searches 6 to 8 (one
-// wave, a chain of scans), the place of the token 5 to 8.  126464 entries: 32 rows 25 us, 256 guided 50 us (2.6 TB/s), 2048
-// rows 191 us (2.7 TB/s).  Tried and dropped: 512 lanes that stream a row and read it again for the token's place, two
-// workgroups a CU (32 rows 37 us against 30 of this form in the same run, 2048 198 / 194, 2048 guided 508 / 344: the second
-// reading costs what the overlap saves); a wave-major order of the chunks (slower).  Not built: a row over several CUs,
-// whose histograms together are as many bytes as the row.
+// Bound by a CU's own work on a row, 49 to 55 thousand cycles where 1024 lanes do it: the histogram 18 to 28 (its LDS
+// atomics alone 16: 64 random bins meet in the banks, 8 cycles an instruction), listing the occupied bins 6, their weights
+// 4, the searches 6 to 8 (one wave, a chain of scans), the place of the token 5 to 8; from a few rows a CU on by memory
+// (Shape).  126464 entries: 32 rows 26 us, 256 guided 50 us (2.6 TB/s), 2048 rows 148 us (3.5 TB/s).
+// Tried and dropped: reading a row twice and keeping none of it (2048 rows 198 us against the 194 of rows kept whole); a
+// wave-major order of the chunks (slower).  Not built: a row over several CUs, whose histograms together are as many bytes
+// as the row.
 #include "common.h"
 #include "philox.h"
 #include "rowregs.h"
 
 namespace {
 
-constexpr int THREADS = ROW_THREADS;                 // 1024
-constexpr int SLOTS = ROW_SLOTS;                     // 16-byte chunks a lane
-constexpr int NWV = THREADS / 64;
-constexpr unsigned MAG_LO = 0x2400, MAG_HI = 0x4380; // magnitudes with a bin of their own: [2^-55, 2^8)
-constexpr int SPAN = MAG_HI - MAG_LO;                // 8064; bin 0: below the range (zero), SPAN + 1: above
-constexpr int NEGATIVE = 0x8000;                     // bin of a negative value: the sign bit stays where it is
-constexpr int REGULAR_KEYS = 2 * SPAN + 1;           // descending values: SPAN positive, zero, SPAN negative
-constexpr int REGULAR_CHUNKS = (REGULAR_KEYS + 63) / 64;
-constexpr int PER_WAVE = 16;                         // groups of 64 keys of a regular row a wave looks through
-static_assert(REGULAR_CHUNKS <= PER_WAVE * NWV && NWV == 16 && PER_WAVE == 16, "every group has a wave");
-constexpr int WINDOW = 16384;                        // irregular rows: keys counted at a time, 4 windows
 constexpr int MAX_CHUNKS = 65536 / 64;
-constexpr int REST_AT = WINDOW;                      // in LDS words: the other shared state, between the planes
-constexpr int LDS_WORDS = NEGATIVE + SPAN + 2;
 constexpr unsigned LLADA_STREAM_SAMPLE = 4u;
 
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
@@ -65,22 +52,53 @@ struct SampleArgs {
     llada_remask_args r;      // remasking epilogue
 };
 
-struct Shared {
-    unsigned cnt[MAX_CHUNKS];        // entries of a chunk of 64 keys, then: entries before it
-    double mass[MAX_CHUNKS];         // their weight, then: the weight before it
-    double conf[NWV];                // epilogue: partial sums of the waves
-    double total_mass;
-    unsigned total;
-    int first[NWV];
-    int irregular;
-    int j, tied;                     // the drawn entry: the j-th of `tied` equal ones
-    float value, prob;
-    unsigned slot_tot[SLOTS / 2];    // two slots a word
-    unsigned wave_tot[NWV];
-    int token;
-    unsigned short patterns[REGULAR_KEYS + 64];   // regular rows: the values that have entries, in order
+// What a workgroup is made for.
+//   WHOLE  1024 lanes keep the row in registers (16 x 16 bytes each), one workgroup a CU: the row is read once.
+//   else   512 lanes keep the first half of the longest row, read the rest past, and read that again only when the drawn
+//          entry is not in the half they hold; half the LDS, so two workgroups share a CU and one's reading goes on under
+//          the other's searches.
+// Both sides, us a call (whole / half): 32 rows 30 / 34, 256 37 / 39, 257 50 / 44, 512 63 / 62, 1024 109 / 99, 2048 198 / 162;
+// with the epilogue 256 rows 37 / 39, 512 68 / 58, 2048 216 / 156.  Guided rows are always kept whole: combining is
+// arithmetic, which a second workgroup does not hide (256 rows 57 / 76, 2048 341 / 372).
+template <bool WHOLE_>
+struct Shape {
+    static constexpr bool WHOLE = WHOLE_;
+    static constexpr int HELD = 16;                                // chunks of 16 bytes a lane keeps
+    static constexpr int THREADS = WHOLE ? 1024 : 512;
+    static constexpr int NWV = THREADS / 64;
+    static constexpr int SLOTS = ROW_MAX_VOCAB / 8 / THREADS;      // 16-byte chunks a lane
+    // magnitudes with a bin of their own: [2^-55, 2^8), or [2^-35, 2^8)
+    static constexpr unsigned MAG_HI = 0x4380, MAG_LO = WHOLE ? 0x2400 : 0x2E00;
+    static constexpr int SPAN = MAG_HI - MAG_LO;                   // bin 0: below the range (zero), SPAN + 1: above
+    // bin of a negative value: the sign bit stays where it is and what is between the planes holds the other shared state,
+    // or the second plane follows the first
+    static constexpr int NEGATIVE = WHOLE ? 0x8000 : SPAN + 2;
+    static constexpr int REGULAR_KEYS = 2 * SPAN + 1;              // descending values: SPAN positive, zero, SPAN negative
+    static constexpr int GROUPS = (REGULAR_KEYS + 63) / 64;
+    static constexpr int PER_WAVE = (GROUPS + NWV - 1) / NWV;      // groups of 64 keys a wave looks through
+    static constexpr int WINDOW = WHOLE ? 16384 : 8192;             // irregular rows: keys counted at a time
+    static constexpr int REST_AT = WHOLE ? WINDOW : (2 * (SPAN + 2) + 3) / 4 * 4;   // in LDS words: the other shared state
+
+    struct Shared {
+        unsigned cnt[MAX_CHUNKS];        // entries of a chunk of 64 positions, then: entries before it
+        double mass[MAX_CHUNKS];         // their weight, then: the weight before it
+        double conf[NWV];                // epilogue: partial sums of the waves
+        double total_mass;
+        unsigned total;
+        int first[NWV];
+        int irregular;
+        int j, tied;                     // the drawn entry: the j-th of `tied` equal ones
+        float value, prob;
+        unsigned slot_tot[SLOTS];
+        unsigned wave_tot[NWV];
+        int token;
+        unsigned short patterns[REGULAR_KEYS + 64];   // regular rows: the values that have entries, in order
+    };
+    static constexpr int LDS_WORDS = WHOLE ? NEGATIVE + SPAN + 2 : REST_AT + (int)((sizeof(Shared) + 3) / 4);
+    static_assert(SPAN % 64 == 0 && REGULAR_KEYS % 64 == 1, "a group's keys have one sign; the last group has one key");
+    static_assert(GROUPS <= 256 && PER_WAVE <= 64 && NWV % 4 == 0 && SLOTS <= 64 && WINDOW <= REST_AT, "ranges of the scans");
+    static_assert(WHOLE ? REST_AT * 4 + sizeof(Shared) <= NEGATIVE * 4 && LDS_WORDS * 4 <= 160 * 1024 : LDS_WORDS * 4 <= 80 * 1024, "LDS");
 };
-static_assert(REST_AT * 4 + sizeof(Shared) <= NEGATIVE * 4 && LDS_WORDS * 4 <= 160 * 1024, "the planes leave room");
 
 // irregular rows: position p of the whole key space (0 = the largest value) -> bf16 pattern
 __device__ __forceinline__ unsigned full_bits(int p) {
@@ -177,11 +195,17 @@ __device__ __forceinline__ u32x4 row_chunk(const bf16_t* lc, const bf16_t* lu, i
     return t;
 }
 
-// One more in the bins of a word's two entries: bin = clamped magnitude, the sign bit in place (in `word`).  The addresses are
-// formed in three instructions by hand (merge the signs, shift either half), where the compiler takes five.
-__device__ __forceinline__ void count_two(unsigned* bins, unsigned word, unsigned clamped) {
+// One more in the bins of a word's two entries.  The addresses are formed by hand where the compiler takes two instructions
+// more for each word.
+template <class L>
+__device__ __forceinline__ void count_two(unsigned* bins, unsigned word) {
+    const u16x2 idx = __builtin_elementwise_min(
+        __builtin_elementwise_sub_sat(halves(word & 0x7FFF7FFFu), (u16x2)((unsigned short)(L::MAG_LO - 1))), (u16x2)((unsigned short)(L::SPAN + 1)));
     unsigned at, lo, hi;
-    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(at) : "v"(word), "s"(0x80008000u), "v"(clamped));
+    if constexpr (L::WHOLE)
+        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(at) : "v"(word), "s"(0x80008000u), "v"(__builtin_bit_cast(unsigned, idx)));
+    else
+        asm("v_pk_mad_u16 %0, %1, %2, %3" : "=v"(at) : "v"(halves(word) >> (unsigned short)15), "v"((unsigned)L::NEGATIVE * 0x00010001u), "v"(idx));
     asm("v_lshlrev_b32_sdwa %0, %2, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:WORD_0" : "=v"(lo) : "v"(at), "v"(2u));
     asm("v_lshlrev_b32_sdwa %0, %2, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:WORD_1" : "=v"(hi) : "v"(at), "v"(2u));
     atomicAdd((unsigned*)((unsigned char*)bins + lo), 1u);
@@ -196,23 +220,26 @@ __device__ __forceinline__ unsigned zero_halves(unsigned x) {
 }
 
 // Draws the token of one row.  EPI: also leaves the row's confidence (rules of llada_remask_scores) in `conf`.
-template <bool EPI>
-__device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
+template <bool EPI, class L>
+__device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, typename L::Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
                                            double top_p, double min_p, double u, int excl_all, int excl_conf, float& conf) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int THREADS = L::THREADS, NWV = L::NWV, SLOTS = L::SLOTS, HELD = L::HELD, SPAN = L::SPAN, NEGATIVE = L::NEGATIVE, WINDOW = L::WINDOW, PER_WAVE = L::PER_WAVE;
+    constexpr int REGULAR_KEYS = L::REGULAR_KEYS, WINDOWS = 65536 / WINDOW;
+    constexpr unsigned MAG_LO = L::MAG_LO, MAG_HI = L::MAG_HI;
     const int V = a.vocab;
-    // The row in registers: chunk c = lane + 1024 i holds entries 8 c - off .. + 7, off = the row's offset from a 16-byte
-    // boundary in entries, so that all but its first and last chunk are one aligned load.
+    // Chunk c = lane + THREADS i (slot i) holds entries 8 c - off .. + 7, off = the row's offset from a 16-byte boundary in
+    // entries, so that all but its first and last chunk are one aligned load.
     const int off = (int)(((uintptr_t)lc >> 1) & 7);
+    if constexpr (!L::WHOLE) lu = nullptr;
     const int chunks = (V + off + 7) / 8;
 
-    for (int i = tid; i < (SPAN + 2 + 3) / 4; i += THREADS) {
-        ((u32x4*)bins)[i] = (u32x4){0u, 0u, 0u, 0u};
-        if (i < (SPAN + 2) / 4) ((u32x4*)(bins + NEGATIVE))[i] = (u32x4){0u, 0u, 0u, 0u};
+    for (int i = tid; i < SPAN + 2; i += THREADS) bins[i] = bins[NEGATIVE + i] = 0u;
+    if (tid < SLOTS) sh.slot_tot[tid] = 0u;
+    if (tid == 0) {
+        sh.irregular = 0;
+        sh.token = -1;
     }
-    if (tid < (SPAN + 2) % 4) bins[NEGATIVE + (SPAN + 2) / 4 * 4 + tid] = 0u;
-    if (tid < SLOTS / 2) sh.slot_tot[tid] = 0u;
-    if (tid == 0) sh.irregular = 0;
 
     __syncthreads();
 
@@ -225,19 +252,33 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     // entries of a key that this softmax sees
     auto seen = [&](unsigned n, float v) { return n - (v == lx_excl ? 1u : 0u); };
 
-    // The row in registers.  A chunk that the row covers only in part (its first or last) is fetched entry by entry, once and
-    // apart from the others: this code runs once a row, and what it costs beside its memory time is its length.
+    // Chunks that are not one load: those the row covers only in part (its first or last) and the one with the entry taken out
+    // of everything.  They are fetched entry by entry, apart from the others: this code runs once a row, and what it costs
+    // beside its memory time is its length.
+    const int odd[3] = {off != 0 ? 0 : -1, ((V + off) & 7) != 0 ? chunks - 1 : -1, EPI && excl_all >= 0 ? (excl_all + off) >> 3 : -1};
+    auto is_odd = [&](int c) { return c == odd[0] || c == odd[1] || (EPI && c == odd[2]); };
+    auto each_odd = [&](auto&& f) {              // f(slot, words) in the lane that holds the chunk
+        if (odd[0] < 0 && odd[1] < 0 && odd[2] < 0) return;
+#pragma unroll 1
+        for (int k = 0; k < 3; ++k) {
+            const int c = k == 0 ? odd[0] : k == 1 ? odd[1] : odd[2];
+            if (c < 0 || c % THREADS != tid || (k > 0 && c == odd[0]) || (k > 1 && c == odd[1])) continue;
+            f(c / THREADS, row_chunk<EPI>(lc, lu, c * 8 - off, V, a.cfg1, excl_all));
+        }
+    };
     const u32x4 ninf = {BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2};
-    u32x4 q[SLOTS];
+
+    // The chunks that are kept,
+    u32x4 q[HELD];
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-        const int c = tid + i * THREADS, v0 = c * 8 - off;
+    for (int i = 0; i < HELD; ++i) {
+        const int v0 = (tid + i * THREADS) * 8 - off;
         q[i] = ninf;
         if (v0 >= 0 && v0 + 8 <= V) q[i] = __builtin_nontemporal_load((const u32x4*)(lc + v0));
     }
     if (lu) {
 #pragma unroll
-        for (int g = 0; g < SLOTS; g += 8) {
+        for (int g = 0; g < HELD; g += 8) {
             u32x4 b[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -251,31 +292,51 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             }
         }
     }
-    if (off != 0 || ((V + off) & 7) != 0 || (EPI && excl_all >= 0)) {
-        const int ex = EPI && excl_all >= 0 ? (excl_all + off) >> 3 : -1;
-#pragma unroll 1
-        for (int k = 0; k < 3; ++k) {
-            const int c = k == 0 ? 0 : k == 1 ? chunks - 1 : ex;
-            if (c < 0 || (c & (THREADS - 1)) != tid) continue;
-            const u32x4 t = row_chunk<EPI>(lc, lu, c * 8 - off, V, a.cfg1, excl_all);
+    each_odd([&](int slot, u32x4 t) {
 #pragma unroll
-            for (int i = 0; i < SLOTS; ++i)
-                if (i == c / THREADS) q[i] = t;
+        for (int i = 0; i < HELD; ++i)
+            if (i == slot) q[i] = t;
+    });
+    // and the rest, read past: f(slot, words) in every lane of the workgroup (-inf where a lane has no chunk, or an odd one, which
+    // comes at the end, in its lane alone), a few loads ahead
+    auto rest = [&](auto&& f) {
+        constexpr int AHEAD = EPI ? 4 : 8;                            // (the epilogue's registers: 8 spill, 2048 rows 156 / 171 us)
+        const int used = (chunks + THREADS - 1) / THREADS;
+        if (HELD == SLOTS || used <= HELD) return;
+        u32x4 next[AHEAD];
+        auto plain = [&](int slot) { return tid + slot * THREADS < chunks && !is_odd(tid + slot * THREADS); };
+        auto fetch = [&](int slot, int i) {
+            next[i] = ninf;
+            if (plain(slot)) next[i] = *(const u32x4*)(lc + ((tid + slot * THREADS) * 8 - off));
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fetch(HELD + i, i);
+#pragma unroll 1
+        for (int i0 = HELD; i0 < used; i0 += AHEAD) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const u32x4 t = next[i];
+                fetch(i0 + AHEAD + i, i);
+                if (i0 + i < used) f(i0 + i, t);
+            }
         }
-    }
+        each_odd([&](int slot, u32x4 t) {
+            if (slot >= HELD) f(slot, t);
+        });
+    };
 
     // ---- the histogram, as the chunks arrive: clamped magnitudes, both signs ----
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
+    for (int i = 0; i < HELD; ++i) {
         if (tid + i * THREADS >= chunks) continue;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const u16x2 mag = halves(q[i][e] & 0x7FFF7FFFu);
-            const u16x2 idx = __builtin_elementwise_min(__builtin_elementwise_sub_sat(mag, (u16x2)((unsigned short)(MAG_LO - 1))),
-                                                        (u16x2)((unsigned short)(SPAN + 1)));
-            count_two(bins, q[i][e], __builtin_bit_cast(unsigned, idx));
-        }
+        for (int e = 0; e < 4; ++e) count_two<L>(bins, q[i][e]);
     }
+    rest([&](int i, u32x4 t) {
+        if (tid + i * THREADS >= chunks) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) count_two<L>(bins, t[e]);
+    });
     __syncthreads();
     if (tid == 0) bins[0] += bins[NEGATIVE];     // zero of either sign (the test below holds before and after)
     // clamped bins that are not empty: zeros and -inf are as good as binned, anything else makes the row irregular
@@ -284,15 +345,18 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         const u16x2 one = {1, 1}, minus_inf = {0xFF80, 0xFF80};
         u16x2 least = {0xFFFF, 0xFFFF}, neg = {0, 0};
         s16x2 pos = {0, 0};
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i)
+        auto look = [&](u32x4 t) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const u16x2 w = halves(q[i][e]);
+                const u16x2 w = halves(t[e]);
                 least = __builtin_elementwise_min(least, (w & (unsigned short)0x7FFF) - one);
                 pos = __builtin_elementwise_max(pos, __builtin_bit_cast(s16x2, w));
                 neg = __builtin_elementwise_max(neg, w * __builtin_elementwise_min(w ^ minus_inf, one));
             }
+        };
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) look(q[i]);
+        rest([&](int, u32x4 t) { look(t); });
         const bool bad = min(least[0], least[1]) < MAG_LO - 1 || (unsigned)max(pos[0], pos[1]) >= MAG_HI ||
                          max(neg[0], neg[1]) >= 0x8000u + MAG_HI;
         if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) sh.irregular = 1;
@@ -335,7 +399,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         const int at = min(p, n_pos - 1);
         const unsigned bits = bits_at(at), mag = bits & 0x7FFFu;
         Entries x;
-        x.n = bins[regular ? (int)((mag < MAG_LO ? 0u : mag - (MAG_LO - 1u)) | (bits & 0x8000u)) : (at & (WINDOW - 1))];
+        x.n = bins[regular ? (int)(mag < MAG_LO ? 0u : mag - (MAG_LO - 1u)) + (bits & 0x8000u ? NEGATIVE : 0) : (at & (WINDOW - 1))];
         if (p >= n_pos) x.n = 0u;
         x.v = __uint_as_float(bits << 16);
         const double dl = (double)x.v - (double)m;
@@ -356,17 +420,16 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
 
     // ---- totals of the chunks: entries, weight ----
     if (regular) {
-        // group g = i * 16 + wave of 64 keys: neighbouring groups, which are full together, are spread over the waves.  A
+        // group g = i * NWV + wave of 64 keys: neighbouring groups, which are full together, are spread over the waves.  A
         // group's keys have one sign; group SPAN / 64 starts with zero, the last group has one key.  (Few instructions a
-        // group: every wave looks through 16 of them.)
-        static_assert(SPAN % 64 == 0 && REGULAR_KEYS % 64 == 1, "groups");
+        // group: every wave looks through 16 of them, or 22.)
         unsigned n[PER_WAVE];
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
             const int g = i * NWV + wave;                    // (uniform)
             const unsigned* at = bins + (g < SPAN / 64 ? SPAN - g * 64 : NEGATIVE + min(g * 64 - SPAN, SPAN - 63));
             n[i] = at[g < SPAN / 64 ? -lane : lane];
-            if (i == PER_WAVE - 1) n[i] = g > REGULAR_KEYS / 64 ? 0u : g == REGULAR_KEYS / 64 ? (lane == 63 ? n[i] : 0u) : n[i];
+            if ((i + 1) * NWV > REGULAR_KEYS / 64) n[i] = g > REGULAR_KEYS / 64 ? 0u : g == REGULAR_KEYS / 64 ? (lane == 63 ? n[i] : 0u) : n[i];
         }
         if (wave == SPAN / 64 % NWV && lane == 0) n[SPAN / 64 / NWV] = bins[0];
         unsigned held = 0;
@@ -377,8 +440,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         }
         if (lane < PER_WAVE) sh.cnt[lane * NWV + wave] = held;
         __syncthreads();
-        // where each group's keys go in the list: a scan over the 256 groups, in every wave
-        const u32x4 g = *(const u32x4*)&sh.cnt[lane * 4];
+        // where each group's keys go in the list: a scan over the groups, in every wave
+        u32x4 g = *(const u32x4*)&sh.cnt[lane * 4];
+        if (lane * 4 >= PER_WAVE * NWV) g = (u32x4){0u, 0u, 0u, 0u};
         const unsigned upto = wave_scan(g[0] + g[1] + g[2] + g[3]);
         n_pos = (int)from_lane(upto, 63);
         unsigned base = upto - (g[0] + g[1] + g[2] + g[3]);
@@ -392,7 +456,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             const int g = i * NWV + wave;
             const unsigned bits = g < SPAN / 64 ? MAG_HI - 1u - g * 64 - lane : g == REGULAR_KEYS / 64 ? 0x8000u + MAG_HI - 1u
                                                                                                   : 0x8000u + MAG_LO - 1u + (g * 64 - SPAN) + lane;
-            if (n[i]) sh.patterns[from_lane(base, 4 * i + (wave >> 2)) + before] = (unsigned short)(bits == 0x8000u + MAG_LO - 1u ? 0u : bits);
+            if (n[i]) sh.patterns[from_lane(base, (i * NWV + wave) >> 2) + before] = (unsigned short)(bits == 0x8000u + MAG_LO - 1u ? 0u : bits);
         }
         __syncthreads();
         if (n_pos > 0) m = value_at(0);
@@ -400,7 +464,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         for (int c = wave; c * 64 < n_pos; c += NWV) total_chunk(c);
     } else {
         bool found = false;
-        for (int win = 0; win < 4; ++win) {
+        for (int win = 0; win < WINDOWS; ++win) {
             count_window(win);
             const int c_lo = win * (WINDOW / 64), c_hi = c_lo + WINDOW / 64;
             if (!found) {
@@ -606,63 +670,18 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     const unsigned pat = bits * 0x00010001u;
     const unsigned msk = bits == 0u ? 0x7FFF7FFFu : 0xFFFFFFFFu;      // zero: either sign
     const bool single = sh.tied == 1;            // (uniform)
-    int slot = -1;                               // the chunk that holds the entry, in the lane that holds it
-    unsigned skip = 0;                           // matches of that chunk before the entry
-    auto differs = [&](int i, int e) { return (q[i][e] ^ pat) & msk; };       // zero in a half: a match
-    if (single) {
-#pragma unroll
-        for (int g = 0; g < SLOTS; g += 4) {     // most waves hold no match: four chunks are ruled out at a time
-            u16x2 least = halves(differs(g, 0));
-#pragma unroll
-            for (int i = 1; i < 16; ++i) least = __builtin_elementwise_min(least, halves(differs(g + i / 4, i & 3)));
-            if (__builtin_amdgcn_ballot_w64(zero_halves(__builtin_bit_cast(unsigned, least)) != 0u) == 0) continue;
-#pragma unroll
-            for (int i = g; i < g + 4; ++i) {
-                u16x2 x = halves(differs(i, 0));
-#pragma unroll
-                for (int e = 1; e < 4; ++e) x = __builtin_elementwise_min(x, halves(differs(i, e)));
-                if (zero_halves(__builtin_bit_cast(unsigned, x)) != 0u) slot = i;
-            }
-        }
-    } else {
-        unsigned mine[SLOTS / 2];                // matches of each chunk, 16 bits each (a slot's row-wide total fits as well)
-#pragma unroll
-        for (int i = 0; i < SLOTS; i += 2) {
-            unsigned n[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                // sums of the packed halves: at most 4 a half
-                const unsigned h = zero_halves(differs(i + k, 0)) + zero_halves(differs(i + k, 1)) + zero_halves(differs(i + k, 2)) +
-                                   zero_halves(differs(i + k, 3));
-                n[k] = (h & 0xFFFFu) + (h >> 16);
-            }
-            mine[i / 2] = n[0] | n[1] << 16;
-            const unsigned sum = wave_scan(mine[i / 2]);
-            if (lane == 63 && sum) atomicAdd(&sh.slot_tot[i / 2], sum);
-        }
-        __syncthreads();
-        const unsigned upto = wave_scan(lane < SLOTS ? (sh.slot_tot[(lane & (SLOTS - 1)) / 2] >> (16 * (lane & 1))) & 0xFFFFu : 0u);
-        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > (unsigned)sh.j));
-        const unsigned left = (unsigned)sh.j - from_lane(lane_before(upto), at);
-        unsigned n_here = 0;
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i)
-            if (i == at) n_here = (mine[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
-        const unsigned incl = wave_scan(n_here);
-        if (lane == 63) sh.wave_tot[wave] = incl;
-        __syncthreads();
-        const unsigned waves = wave_scan(lane < NWV ? sh.wave_tot[lane & (NWV - 1)] : 0u);
-        const unsigned before = from_lane(lane_before(waves), wave) + incl - n_here;
-        if (left >= before && left < before + n_here) {
-            slot = at;
-            skip = left - before;
-        }
-    }
-    if (slot >= 0) {
-        u32x4 t = q[0];
-#pragma unroll
-        for (int i = 1; i < SLOTS; ++i)
-            if (i == slot) t = q[i];
+    auto differs = [&](unsigned w) { return (w ^ pat) & msk; };               // zero in a half: a match
+    auto nearest = [&](u32x4 t) {                                             // zero in a half: a match in that half of some word
+        return __builtin_elementwise_min(__builtin_elementwise_min(halves(differs(t[0])), halves(differs(t[1]))),
+                                         __builtin_elementwise_min(halves(differs(t[2])), halves(differs(t[3]))));
+    };
+    auto any_match = [](u16x2 least) { return zero_halves(__builtin_bit_cast(unsigned, least)) != 0u; };
+    auto matches = [&](u32x4 t) {                                             // sums of the packed halves: at most 4 a half
+        const unsigned h = zero_halves(differs(t[0])) + zero_halves(differs(t[1])) + zero_halves(differs(t[2])) + zero_halves(differs(t[3]));
+        return (h & 0xFFFFu) + (h >> 16);
+    };
+    // the token: the entry of chunk `slot` of this lane that matches after `skip` others
+    auto take = [&](u32x4 t, int slot, unsigned skip) {
         unsigned ahead = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -670,6 +689,69 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             if (match && ahead == skip) sh.token = (tid + slot * THREADS) * 8 - off + e;
             ahead += match;
         }
+    };
+    const bool more = HELD < SLOTS && chunks > HELD * THREADS;                // (uniform)
+    if (single) {
+        int slot = -1;
+#pragma unroll
+        for (int g = 0; g < HELD; g += 4) {      // most waves hold no match: four chunks are ruled out at a time
+            u16x2 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = nearest(q[g + i]);
+            if (__builtin_amdgcn_ballot_w64(any_match(__builtin_elementwise_min(__builtin_elementwise_min(x[0], x[1]), __builtin_elementwise_min(x[2], x[3])))) == 0) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (any_match(x[i])) slot = g + i;
+        }
+        if (slot >= 0) {
+            u32x4 t = q[0];
+#pragma unroll
+            for (int i = 1; i < HELD; ++i)
+                if (i == slot) t = q[i];
+            take(t, slot, 0u);
+        }
+        if (more) {
+            __syncthreads();
+            if (sh.token < 0)
+                rest([&](int i, u32x4 t) {
+                    if (any_match(nearest(t))) take(t, i, 0u);
+                });
+        }
+    } else {
+        // matches of every slot, row-wide; then of the lanes of the slot that holds the entry
+#pragma unroll
+        for (int i = 0; i < HELD; i += 2) {      // (two slots' totals in one scan, 16 bits each)
+            const unsigned sum = wave_scan(matches(q[i]) | matches(q[i + 1]) << 16);
+            if (lane == 63 && sum) {
+                atomicAdd(&sh.slot_tot[i], sum & 0xFFFFu);
+                atomicAdd(&sh.slot_tot[i + 1], sum >> 16);
+            }
+        }
+        __syncthreads();
+        unsigned upto = wave_scan(lane < SLOTS ? sh.slot_tot[lane & (SLOTS - 1)] : 0u);
+        if (more && from_lane(upto, 63) <= (unsigned)sh.j) {      // (uniform)
+            __syncthreads();
+            rest([&](int i, u32x4 t) {
+                const unsigned n = matches(t);
+                if (n) atomicAdd(&sh.slot_tot[i], n);
+            });
+            __syncthreads();
+            upto = wave_scan(lane < SLOTS ? sh.slot_tot[lane & (SLOTS - 1)] : 0u);
+        }
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > (unsigned)sh.j));
+        const unsigned left = (unsigned)sh.j - from_lane(lane_before(upto), at);
+        u32x4 here = ninf;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (i == at) here = q[i];
+        if (at >= HELD && tid + at * THREADS < chunks) here = row_chunk<EPI>(lc, lu, (tid + at * THREADS) * 8 - off, V, a.cfg1, excl_all);
+        const unsigned n_here = matches(here);
+        const unsigned incl = wave_scan(n_here);
+        if (lane == 63) sh.wave_tot[wave] = incl;
+        __syncthreads();
+        const unsigned waves = wave_scan(lane < NWV ? sh.wave_tot[lane & (NWV - 1)] : 0u);
+        const unsigned before = from_lane(lane_before(waves), wave) + incl - n_here;
+        if (left >= before && left < before + n_here) take(here, at, left - before);
     }
     __syncthreads();
 
@@ -697,7 +779,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
                 const float p = round_bf16((float)(exp(dl) / S)), lp = round_bf16((float)(dl - lse));
                 return (double)round_bf16(lp * p);
             };
-            for (int win = 0; win < (regular ? 1 : 4); ++win) {
+            for (int win = 0; win < (regular ? 1 : WINDOWS); ++win) {
                 if (!regular) count_window(win);
                 const int p_lo = regular ? 0 : win * WINDOW, p_hi = regular ? n_pos : p_lo + WINDOW;
 #pragma unroll 1
@@ -720,10 +802,11 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
 }
 
 // One workgroup per row.
-template <bool EPI>
-__global__ void __launch_bounds__(THREADS) sample_rows_kernel(const SampleArgs a) {
-    __shared__ __attribute__((aligned(16))) unsigned lds[LDS_WORDS];
-    Shared& sh = *(Shared*)(lds + REST_AT);
+template <bool EPI, bool WHOLE>
+__global__ void __launch_bounds__(Shape<WHOLE>::THREADS, 4) sample_rows_kernel(const SampleArgs a) {
+    using L = Shape<WHOLE>;
+    __shared__ __attribute__((aligned(16))) unsigned lds[L::LDS_WORDS];
+    typename L::Shared& sh = *(typename L::Shared*)(lds + L::REST_AT);
     const int row = blockIdx.x;
     const int tid = threadIdx.x;
     int pos = row, b = row, col = 0;
@@ -751,7 +834,7 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const SampleArgs a
     const int ex_all = EPI && (a.r.flags & LLADA_FLAG_LOGITS_EOS_INF) ? a.r.eos_id : -1;
     const int ex_conf = EPI && (a.r.flags & LLADA_FLAG_CONF_EOS_EOT_INF) && a.r.eot_id != ex_all ? a.r.eot_id : -1;
     float conf = 0.f;
-    sample_row<EPI>(a, lds, sh, lc, lu, T, top_k, top_p, min_p, u, ex_all, ex_conf, conf);
+    sample_row<EPI, L>(a, lds, sh, lc, lu, T, top_k, top_p, min_p, u, ex_all, ex_conf, conf);
     if (tid != 0) return;
     if constexpr (EPI) {
         if (a.r.remasking == LLADA_REMASK_RANDOM) {
@@ -781,6 +864,18 @@ __global__ void __launch_bounds__(256) sample_defaults_kernel(const int64_t* __r
     }
 }
 
+int g_force = 0;        // test hook
+
+// One workgroup a row, of the kind that pays (Shape).
+template <bool EPI>
+void launch_rows(const SampleArgs& a, int n_rows, hipStream_t st) {
+    const bool half = a.uncond == nullptr && (g_force ? g_force == 2 : n_rows > 256);
+    if (half)
+        hipLaunchKernelGGL((sample_rows_kernel<EPI, false>), dim3(n_rows), dim3(Shape<false>::THREADS), 0, st, a);
+    else
+        hipLaunchKernelGGL((sample_rows_kernel<EPI, true>), dim3(n_rows), dim3(Shape<true>::THREADS), 0, st, a);
+}
+
 int check_sampling(const char* who, const llada_sampling* s) {
     LLADA_CHECK_ARG(s != nullptr, "%s: null sampling parameters", who);
     LLADA_CHECK_ARG(s->row_temperature || (s->temperature >= 0.0 && s->temperature <= 1.0e30), "%s: temperature %g", who, s->temperature);
@@ -791,6 +886,9 @@ int check_sampling(const char* who, const llada_sampling* s) {
 }
 
 }  // namespace
+
+// tests: rows kept whole (1), kept by half where that is possible (2); 0 = automatic
+extern "C" void llada_sample_rows_force(int kind) { g_force = kind; }
 
 extern "C" int llada_sample_rows(const void* logits, const void* uncond_logits, int64_t row_stride, double cfg_scale,
                                  int32_t n_rows, int32_t vocab, const llada_sampling* sampling, uint64_t seed, uint32_t step,
@@ -816,7 +914,7 @@ extern "C" int llada_sample_rows(const void* logits, const void* uncond_logits, 
     a.row_offset = row_offset;
     a.tokens = tokens;
     a.probs = probs;
-    hipLaunchKernelGGL(sample_rows_kernel<false>, dim3(n_rows), dim3(THREADS), 0, (hipStream_t)stream, a);
+    launch_rows<false>(a, n_rows, (hipStream_t)stream);
     LLADA_CHECK_LAUNCH("sample_rows_kernel");
     return LLADA_OK;
 }
@@ -854,7 +952,7 @@ extern "C" int llada_remask_scores_sampled(const llada_remask_args* args, const 
     a.step = r.step;
     a.row_offset = r.row_offset;
     a.r = r;
-    hipLaunchKernelGGL(sample_rows_kernel<true>, dim3(r.n_rows), dim3(THREADS), 0, st, a);
+    launch_rows<true>(a, r.n_rows, st);
     LLADA_CHECK_LAUNCH("sample_rows_kernel");
     return LLADA_OK;
 }

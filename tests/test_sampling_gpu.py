@@ -12,6 +12,14 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 
+@pytest.fixture(params=["whole", "half"])
+def lib(lib, request):
+    """Every test of this file with both kinds of workgroup."""
+    lib.llada_sample_rows_force(1 if request.param == "whole" else 2)
+    yield lib
+    lib.llada_sample_rows_force(0)
+
+
 def bf16(a):
     return torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)).cuda().to(torch.bfloat16)
 
@@ -272,3 +280,31 @@ def test_top_k_past_32_bits_keeps_the_row(lib):
     assert torch.equal(sample_tokens(x, top_k=torch.full((6,), 2 ** 32 + 1, device="cuda"), uniforms=u), want)
     with pytest.raises(AssertionError):
         sample_tokens(x, top_k=5 - 2 ** 32, uniforms=u)
+
+
+@pytest.mark.parametrize("V", [9000, 126464])
+def test_the_rule_picks_a_kind_that_gives_the_same(lib, V):
+    from llada_amd import sample_tokens
+    n = 259
+    x, u = logits(95, n, V), uniforms(95, n)
+    forced = [t.clone() for t in sample_tokens(x, 0.9, 40, 0.9, 0.01, uniforms=torch.from_numpy(u).cuda(), return_probs=True)]
+    lib.llada_sample_rows_force(0)
+    for k in (n, 256):
+        tok, pr = sample_tokens(x[:k], 0.9, 40, 0.9, 0.01, uniforms=torch.from_numpy(u[:k]).cuda(), return_probs=True)
+        assert torch.equal(tok, forced[0][:k]) and torch.equal(pr, forced[1][:k])
+    check(x[:12], u[:12], temperature=0.9, top_k=40, top_p=0.9, min_p=0.01)
+
+
+def test_ties_and_the_last_entry_of_a_long_row(lib):
+    # the drawn entry in each chunk of the row, among few equal ones and among very many
+    V = 131072
+    places = list(range(0, V, 4099)) + [V - 1]
+    x = torch.full((len(places), V), -3.0)
+    for r, at in enumerate(places):
+        x[r, at] = 8.0
+    from llada_amd import sample_tokens
+    tok = sample_tokens(x.cuda().to(torch.bfloat16), top_k=1)
+    assert tok.tolist() == places
+    flat = torch.full((len(places), V), 0.5).cuda().to(torch.bfloat16)
+    u = (np.array(places) + 0.5) / V
+    assert sample_tokens(flat, uniforms=torch.from_numpy(u).cuda()).tolist() == places
