@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
     for (int buf = 0; f_next < f_end; f_next += AHEAD) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // this wave's pieces have landed
         __syncthreads();                                                // everyone's
-        const int f = NK == 1 ? f_next : f_next + ((kg + u_begin - f_next) & (NK - 1));     // the tile of this round that is this wave's
+        const int f = NK == 1 ? f_next : f_next + ((kg + u_begin - f_next) & (NK - 1));     // this wave's tile of the two
         const int f0 = f * KV8_TOKENS;
         if (NK == 1 && f + 1 < f_end) fetch_fresh(f + 1, buf ^ 1);      // (the buffer of the last round is no longer read)
         if (!idle && f < min(f_next + AHEAD, f_end)) {

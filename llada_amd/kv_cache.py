@@ -41,7 +41,6 @@ class KVCache8:
         self._index = self.device.index
         n_tiles = n_seq * n_heads * ((seq_len + 63) // 64)
         self.data[:, :n_tiles * 8].view(torch.float32).fill_(1.0)      # the scales of all-zero blocks
-        self._base = self.data.data_ptr()
         self._ws_bytes = {}
 
     def numel_bytes(self):
@@ -51,7 +50,7 @@ class KVCache8:
     def _layer(self, layer):
         if not 0 <= layer < self.n_layers:
             raise IndexError(f"layer {layer} of a cache of {self.n_layers}")
-        return self._base + layer * self.layer_bytes
+        return self.data.data_ptr() + layer * self.layer_bytes
 
     def _rows(self, x, n, width, what):
         """x as n rows a sequence at one row stride: (tensor kept alive, row stride)."""

@@ -30,7 +30,8 @@ def scalar_sampling(temperature, top_k, top_p, min_p, uniforms=None):
 
 def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uniforms=None, uncond_logits=None, cfg_scale=0.0,
                   seed=0, step=0, row_offset=0, return_probs=False):
-    """One token id per row of ``logits`` [..., vocab] (bf16), int64 [...].
+    """One token id per row of ``logits`` [..., vocab] (bf16, vocab up to 131072, or 131065 where the rows do not start at
+    16-byte boundaries), int64 [...].
 
     With a row's entries ordered by (logit descending, index ascending) and w_i = exp((l_i - max) / temperature) in
     float64: top-k keeps the first ``top_k`` (0: all), top-p the shortest prefix of those with at least ``top_p`` of
