@@ -22,7 +22,7 @@
 // Bound by a CU's own work on a row, 49 to 55 thousand cycles where 1024 lanes do it: the histogram 18 to 28 (its LDS
 // atomics alone 16: 64 random bins meet in the banks, 8 cycles an instruction), listing the occupied bins 6, their weights
 // 4, the searches 6 to 8 (one wave, a chain of scans), the place of the token 5 to 8; from a few rows a CU on by memory
-// (Shape).  126464 entries: 32 rows 26 us, 256 guided 50 us (2.6 TB/s), 2048 rows 148 us (3.5 TB/s).
+// (Shape).  126464 entries: 32 rows 26 us, 256 guided 50 us (2.6 TB/s), 2048 rows 148 us (3.5 TB/s of rows).
 // Tried and dropped: reading a row twice and keeping none of it (2048 rows 198 us against the 194 of rows kept whole); a
 // wave-major order of the chunks (slower).  Not built: a row over several CUs, whose histograms together are as many bytes
 // as the row.
@@ -57,9 +57,9 @@ struct SampleArgs {
 //   else   512 lanes keep the first half of the longest row, read the rest past, and read that again only when the drawn
 //          entry is not in the half they hold; half the LDS, so two workgroups share a CU and one's reading goes on under
 //          the other's searches.
-// Both sides, us a call (whole / half): 32 rows 30 / 34, 256 37 / 39, 257 50 / 44, 512 63 / 62, 1024 109 / 99, 2048 198 / 162;
-// with the epilogue 256 rows 37 / 39, 512 68 / 58, 2048 216 / 156.  Guided rows are always kept whole: combining is
-// arithmetic, which a second workgroup does not hide (256 rows 57 / 76, 2048 341 / 372).
+// Both sides, us a call (whole / half): 32 rows 30 / 35, 256 34 / 41, 257 49 / 43, 512 60 / 62, 1024 105 / 99, 2048 191 / 163;
+// with the epilogue 256 rows 36 / 39, 512 66 / 58, 2048 209 / 157.  Guided rows are always kept whole: combining is
+// arithmetic, which a second workgroup does not hide (256 rows 57 / 76, 2048 341 / 372 when both existed).
 template <bool WHOLE_>
 struct Shape {
     static constexpr bool WHOLE = WHOLE_;
@@ -169,11 +169,18 @@ constexpr double LOG2E = 1.44269504088896340736;
 // (by value: a bit cast straight from a vector's element reads the vector's first)
 __device__ __forceinline__ u16x2 halves(unsigned w) { return __builtin_bit_cast(u16x2, w); }
 
-// generate.py:89-90 on eight entries
+// generate.py:89-90 on eight entries: cfg_combine's three operations, each rounded to bf16, two entries a conversion (17
+// instructions for two entries instead of 26: guided rows are bound by them)
 __device__ __forceinline__ u32x4 combine(u32x4 c, u32x4 u, float cfg1) {
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    auto rounded = [](float lo, float hi) { return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){lo, hi}, bf16x2)); };
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        c[e] = pack_bf16x2(cfg_combine(bf16lo(c[e]), bf16lo(u[e]), cfg1), cfg_combine(bf16hi(c[e]), bf16hi(u[e]), cfg1));
+    for (int e = 0; e < 4; ++e) {
+        unsigned d = rounded(bf16lo(c[e]) - bf16lo(u[e]), bf16hi(c[e]) - bf16hi(u[e]));
+        d = rounded(bf16lo(d) * cfg1, bf16hi(d) * cfg1);
+        c[e] = rounded(bf16lo(u[e]) + bf16lo(d), bf16hi(u[e]) + bf16hi(d));
+    }
     return c;
 }
 
@@ -220,7 +227,7 @@ __device__ __forceinline__ unsigned zero_halves(unsigned x) {
 }
 
 // Draws the token of one row.  EPI: also leaves the row's confidence (rules of llada_remask_scores) in `conf`.
-template <bool EPI, class L>
+template <bool EPI, class L, bool GUIDED>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, typename L::Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
                                            double top_p, double min_p, double u, int excl_all, int excl_conf, float& conf) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -231,7 +238,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     // Chunk c = lane + THREADS i (slot i) holds entries 8 c - off .. + 7, off = the row's offset from a 16-byte boundary in
     // entries, so that all but its first and last chunk are one aligned load.
     const int off = (int)(((uintptr_t)lc >> 1) & 7);
-    if constexpr (!L::WHOLE) lu = nullptr;
+    if constexpr (!GUIDED) lu = nullptr;
     const int chunks = (V + off + 7) / 8;
 
     for (int i = tid; i < SPAN + 2; i += THREADS) bins[i] = bins[NEGATIVE + i] = 0u;
@@ -266,6 +273,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             f(c / THREADS, row_chunk<EPI>(lc, lu, c * 8 - off, V, a.cfg1, excl_all));
         }
     };
+    // (a uniform address and one 32-bit offset for all slots)
+    auto chunk_at = [&](const bf16_t* row, int slot) { return (const u32x4*)((const char*)(row - off) + (size_t)slot * (THREADS * 16) + (unsigned)tid * 16u); };
     const u32x4 ninf = {BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2, BF16_NEG_INF2};
 
     // The chunks that are kept,
@@ -274,29 +283,14 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     for (int i = 0; i < HELD; ++i) {
         const int v0 = (tid + i * THREADS) * 8 - off;
         q[i] = ninf;
-        if (v0 >= 0 && v0 + 8 <= V) q[i] = __builtin_nontemporal_load((const u32x4*)(lc + v0));
-    }
-    if (lu) {
-#pragma unroll
-        for (int g = 0; g < HELD; g += 8) {
-            u32x4 b[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int v0 = (tid + (g + i) * THREADS) * 8 - off;
-                if (v0 >= 0 && v0 + 8 <= V) b[i] = __builtin_nontemporal_load((const u32x4*)(lu + v0));
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int v0 = (tid + (g + i) * THREADS) * 8 - off;
-                if (v0 >= 0 && v0 + 8 <= V) q[g + i] = combine(q[g + i], b[i], a.cfg1);
-            }
-        }
+        if (v0 >= 0 && v0 + 8 <= V) q[i] = __builtin_nontemporal_load(chunk_at(lc, i));
     }
     each_odd([&](int slot, u32x4 t) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
             if (i == slot) q[i] = t;
     });
+    auto plain = [&](int slot) { return tid + slot * THREADS < chunks && !is_odd(tid + slot * THREADS); };
     // and the rest, read past: f(slot, words) in every lane of the workgroup (-inf where a lane has no chunk, or an odd one, which
     // comes at the end, in its lane alone), a few loads ahead
     auto rest = [&](auto&& f) {
@@ -304,10 +298,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         const int used = (chunks + THREADS - 1) / THREADS;
         if (HELD == SLOTS || used <= HELD) return;
         u32x4 next[AHEAD];
-        auto plain = [&](int slot) { return tid + slot * THREADS < chunks && !is_odd(tid + slot * THREADS); };
         auto fetch = [&](int slot, int i) {
             next[i] = ninf;
-            if (plain(slot)) next[i] = *(const u32x4*)(lc + ((tid + slot * THREADS) * 8 - off));
+            if (plain(slot)) next[i] = *chunk_at(lc, slot);
         };
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) fetch(HELD + i, i);
@@ -326,11 +319,33 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     };
 
     // ---- the histogram, as the chunks arrive: clamped magnitudes, both signs ----
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        if (tid + i * THREADS >= chunks) continue;
+    auto count = [&](int i) {
+        if (tid + i * THREADS >= chunks) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e) count_two<L>(bins, q[i][e]);
+    };
+    if constexpr (GUIDED) {            // eight chunks of the other row are on their way while the eight before are counted
+        u32x4 b[8];
+        auto fetch = [&](int g) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (plain(g + i)) b[i] = __builtin_nontemporal_load(chunk_at(lu, g + i));
+        };
+        fetch(0);
+#pragma unroll
+        for (int g = 0; g < HELD; g += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (plain(g + i)) q[g + i] = combine(q[g + i], b[i], a.cfg1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (g + 8 < HELD) fetch(g + 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) count(g + i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) count(i);
     }
     rest([&](int i, u32x4 t) {
         if (tid + i * THREADS >= chunks) return;
@@ -802,7 +817,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
 }
 
 // One workgroup per row.
-template <bool EPI, bool WHOLE>
+template <bool EPI, bool WHOLE, bool GUIDED>
 __global__ void __launch_bounds__(Shape<WHOLE>::THREADS, 4) sample_rows_kernel(const SampleArgs a) {
     using L = Shape<WHOLE>;
     __shared__ __attribute__((aligned(16))) unsigned lds[L::LDS_WORDS];
@@ -834,7 +849,7 @@ __global__ void __launch_bounds__(Shape<WHOLE>::THREADS, 4) sample_rows_kernel(c
     const int ex_all = EPI && (a.r.flags & LLADA_FLAG_LOGITS_EOS_INF) ? a.r.eos_id : -1;
     const int ex_conf = EPI && (a.r.flags & LLADA_FLAG_CONF_EOS_EOT_INF) && a.r.eot_id != ex_all ? a.r.eot_id : -1;
     float conf = 0.f;
-    sample_row<EPI, L>(a, lds, sh, lc, lu, T, top_k, top_p, min_p, u, ex_all, ex_conf, conf);
+    sample_row<EPI, L, GUIDED>(a, lds, sh, lc, lu, T, top_k, top_p, min_p, u, ex_all, ex_conf, conf);
     if (tid != 0) return;
     if constexpr (EPI) {
         if (a.r.remasking == LLADA_REMASK_RANDOM) {
@@ -871,9 +886,11 @@ template <bool EPI>
 void launch_rows(const SampleArgs& a, int n_rows, hipStream_t st) {
     const bool half = a.uncond == nullptr && (g_force ? g_force == 2 : n_rows > 256);
     if (half)
-        hipLaunchKernelGGL((sample_rows_kernel<EPI, false>), dim3(n_rows), dim3(Shape<false>::THREADS), 0, st, a);
+        hipLaunchKernelGGL((sample_rows_kernel<EPI, false, false>), dim3(n_rows), dim3(Shape<false>::THREADS), 0, st, a);
+    else if (a.uncond == nullptr)
+        hipLaunchKernelGGL((sample_rows_kernel<EPI, true, false>), dim3(n_rows), dim3(Shape<true>::THREADS), 0, st, a);
     else
-        hipLaunchKernelGGL((sample_rows_kernel<EPI, true>), dim3(n_rows), dim3(Shape<true>::THREADS), 0, st, a);
+        hipLaunchKernelGGL((sample_rows_kernel<EPI, true, true>), dim3(n_rows), dim3(Shape<true>::THREADS), 0, st, a);
 }
 
 int check_sampling(const char* who, const llada_sampling* s) {
