@@ -20,7 +20,9 @@
 // 55 us and 256 on 16 x 2176 169 us (0.59 and 0.86 PFLOP/s: the chain again, two waves a SIMD; 1.5 rounds of workgroups
 // in the former).  Tried and dropped: workgroups of 8 waves (level or slower, but for 64 queries on 8 x 1150: 25.0 us against
 // the 27.5 of that time), a fresh tile in halves of 32 keys with one half's exponentials under the other's products
-// (level; on cached tiles its registers spill), raised wave priority around the products (level).
+// (level; on cached tiles its registers spill), raised wave priority around the products (level), fresh tiles last (a
+// seventh slower), the next values fetched before the next keys are waited for (256 queries on 16 x 2176 166 / 161 us,
+// but 32 on 8 x 384 7.8 / 8.3 and 32 on 1 x 4096 21.8 / 23.4).
 //
 // Scores, running maximum, sums and outputs are float32; P is rounded to bf16 once for the matrix unit, like the keys' and
 // values' bf16 forms it multiplies (at most 2^-8 of a term, averaged over the terms).

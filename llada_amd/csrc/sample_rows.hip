@@ -22,7 +22,7 @@
 // Bound by a CU's own work on a row, 49 to 55 thousand cycles where 1024 lanes do it: the histogram 18 to 28 (its LDS
 // atomics alone 16: 64 random bins meet in the banks, 8 cycles an instruction), listing the occupied bins 6, their weights
 // 4, the searches 6 to 8 (one wave, a chain of scans), the place of the token 5 to 8; from a few rows a CU on by memory
-// (Shape).  126464 entries: 32 rows 26 us, 256 guided 50 us (2.6 TB/s), 2048 rows 148 us (3.5 TB/s of rows).
+// (Shape).  126464 entries: 32 rows 26 us, 256 guided 48 us (2.7 TB/s), 2048 rows 148 us (3.5 TB/s of rows).
 // Tried and dropped: reading a row twice and keeping none of it (2048 rows 198 us against the 194 of rows kept whole); a
 // wave-major order of the chunks (slower).  Not built: a row over several CUs, whose histograms together are as many bytes
 // as the row.
