@@ -110,8 +110,7 @@ class KVCache8:
         """The values ``layer`` stands for: (keys, values), bf16 [n_seq, seq_len, n_heads, 128]."""
         at = self._layer(layer)
         with self._on_device():
-            out = torch.empty((2, self.n_seq, self.seq_len, self.n_heads, HEAD_DIM), dtype=torch.bfloat16, device=self.device)
-            k, v = out[0], out[1]
+            k, v = torch.empty((2, self.n_seq, self.seq_len, self.n_heads, HEAD_DIM), dtype=torch.bfloat16, device=self.device).unbind(0)
             _lib.check(self.lib.llada_kv8_read(at, self._type, k.data_ptr(), v.data_ptr(), self.n_seq, self.seq_len,
                                                self.n_heads, _lib.stream_ptr(self._index)))
         return k, v
