@@ -19,13 +19,14 @@
 // so, at no cost to other rows) and is counted over the whole 16-bit key space in windows instead; -inf entries, NaNs
 // included, have no weight and are never drawn.  A row with nothing else gives token 0 with probability 0.
 //
-// Bound by a CU's own work on a row, 49 to 55 thousand cycles where 1024 lanes do it: the histogram 18 to 28 (its LDS
+// Bound by a CU's own work on a row, 43 to 54 thousand cycles where 1024 lanes do it: the histogram 21 to 27 (its LDS
 // atomics alone 16: 64 random bins meet in the banks, 8 cycles an instruction), listing the occupied bins 6, their weights
-// 4, the searches 6 to 8 (one wave, a chain of scans), the place of the token 5 to 8; from a few rows a CU on by memory
-// (Shape).  126464 entries: 32 rows 26 us, 256 guided 48 us (2.7 TB/s), 2048 rows 148 us (3.5 TB/s of rows).
+// and prefixes 5, the searches 6 (one wave, a chain of scans), the place of the token 3 to 8; from a few rows a CU on by
+// memory (Shape).  126464 entries: 32 rows 26 us, 256 guided 48 us (2.7 TB/s), 2048 rows 148 us (3.5 TB/s of rows).
 // Tried and dropped: reading a row twice and keeping none of it (2048 rows 198 us against the 194 of rows kept whole); a
-// wave-major order of the chunks (slower).  Not built: a row over several CUs, whose histograms together are as many bytes
-// as the row.
+// wave-major order of the chunks (slower); four workgroups that count a quarter of a row each and a fifth that joins
+// their bins and goes on (32 rows 23.4 us against 23.3 in a graph, guided 44 / 39: the second launch and the fixed
+// 20 thousand cycles behind the histogram eat what the counting saves).
 #include "common.h"
 #include "philox.h"
 #include "rowregs.h"
