@@ -58,9 +58,10 @@ struct SampleArgs {
 //   else   512 lanes keep the first half of the longest row, read the rest past, and read that again only when the drawn
 //          entry is not in the half they hold; half the LDS, so two workgroups share a CU and one's reading goes on under
 //          the other's searches.
-// Both sides, us a call (whole / half): 32 rows 30 / 35, 256 34 / 41, 257 49 / 43, 512 60 / 62, 1024 105 / 99, 2048 191 / 163;
-// with the epilogue 256 rows 36 / 39, 512 66 / 58, 2048 209 / 157.  Guided rows are always kept whole: combining is
-// arithmetic, which a second workgroup does not hide (256 rows 57 / 76, 2048 341 / 372 when both existed).
+// Both sides, us a call (whole / half): 256 rows 33 / 39, 512 57 / 59, 1024 99 / 98, 1536 138 / 130, 2048 178 / 161: by half
+// from there on; with the epilogue 256 rows 34 / 38, 512 61 / 56, 2048 194 / 148: past one row a CU.  Guided rows are
+// always kept whole: combining is arithmetic, which a second workgroup does not hide (256 rows 57 / 76, 2048 341 / 372 when
+// both existed).
 template <bool WHOLE_>
 struct Shape {
     static constexpr bool WHOLE = WHOLE_;
@@ -73,12 +74,11 @@ struct Shape {
     static constexpr int SPAN = MAG_HI - MAG_LO;                   // bin 0: below the range (zero), SPAN + 1: above
     // bin of a negative value: the sign bit stays where it is and what is between the planes holds the other shared state,
     // or the second plane follows the first
-    static constexpr int NEGATIVE = WHOLE ? 0x8000 : SPAN + 2;
+    static constexpr int NEGATIVE = WHOLE ? 0x8000 : (SPAN + 2 + 3) / 4 * 4;
     static constexpr int REGULAR_KEYS = 2 * SPAN + 1;              // descending values: SPAN positive, zero, SPAN negative
-    static constexpr int GROUPS = (REGULAR_KEYS + 63) / 64;
-    static constexpr int PER_WAVE = (GROUPS + NWV - 1) / NWV;      // groups of 64 keys a wave looks through
+    static constexpr int RUN = WHOLE ? 16 : 24;                    // neighbouring bins a lane lists: half of the lanes a sign
     static constexpr int WINDOW = WHOLE ? 16384 : 8192;             // irregular rows: keys counted at a time
-    static constexpr int REST_AT = WHOLE ? WINDOW : (2 * (SPAN + 2) + 3) / 4 * 4;   // in LDS words: the other shared state
+    static constexpr int REST_AT = WHOLE ? WINDOW : NEGATIVE + (SPAN + 2 + 3) / 4 * 4;   // in LDS words: the other shared state
 
     struct Shared {
         unsigned cnt[MAX_CHUNKS];        // entries of a chunk of 64 positions, then: entries before it
@@ -95,9 +95,9 @@ struct Shape {
         int token;
         unsigned short patterns[REGULAR_KEYS + 64];   // regular rows: the values that have entries, in order
     };
-    static constexpr int LDS_WORDS = WHOLE ? NEGATIVE + SPAN + 2 : REST_AT + (int)((sizeof(Shared) + 3) / 4);
-    static_assert(SPAN % 64 == 0 && REGULAR_KEYS % 64 == 1, "a group's keys have one sign; the last group has one key");
-    static_assert(GROUPS <= 256 && PER_WAVE <= 64 && NWV % 4 == 0 && SLOTS <= 64 && WINDOW <= REST_AT, "ranges of the scans");
+    static constexpr int LDS_WORDS = WHOLE ? NEGATIVE + (SPAN + 2 + 3) / 4 * 4 : REST_AT + (int)((sizeof(Shared) + 3) / 4);
+    static_assert(RUN % 4 == 0 && SPAN % 4 == 0 && NEGATIVE % 4 == 0 && (SPAN / RUN + 1) <= THREADS / 2, "a lane's run");
+    static_assert((REGULAR_KEYS + 63) / 64 <= 256 && SLOTS <= 64 && WINDOW <= REST_AT, "ranges of the scans");
     static_assert(WHOLE ? REST_AT * 4 + sizeof(Shared) <= NEGATIVE * 4 && LDS_WORDS * 4 <= 160 * 1024 : LDS_WORDS * 4 <= 80 * 1024, "LDS");
 };
 
@@ -232,8 +232,8 @@ template <bool EPI, class L, bool GUIDED>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, typename L::Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
                                            double top_p, double min_p, double u, int excl_all, int excl_conf, float& conf) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    constexpr int THREADS = L::THREADS, NWV = L::NWV, SLOTS = L::SLOTS, HELD = L::HELD, SPAN = L::SPAN, NEGATIVE = L::NEGATIVE, WINDOW = L::WINDOW, PER_WAVE = L::PER_WAVE;
-    constexpr int REGULAR_KEYS = L::REGULAR_KEYS, WINDOWS = 65536 / WINDOW;
+    constexpr int THREADS = L::THREADS, NWV = L::NWV, SLOTS = L::SLOTS, HELD = L::HELD, SPAN = L::SPAN, NEGATIVE = L::NEGATIVE, WINDOW = L::WINDOW, RUN = L::RUN;
+    constexpr int WINDOWS = 65536 / WINDOW;
     constexpr unsigned MAG_LO = L::MAG_LO, MAG_HI = L::MAG_HI;
     const int V = a.vocab;
     // Chunk c = lane + THREADS i (slot i) holds entries 8 c - off .. + 7, off = the row's offset from a 16-byte boundary in
@@ -295,7 +295,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     // and the rest, read past: f(slot, words) in every lane of the workgroup (-inf where a lane has no chunk, or an odd one, which
     // comes at the end, in its lane alone), a few loads ahead
     auto rest = [&](auto&& f) {
-        constexpr int AHEAD = EPI ? 4 : 8;                            // (the epilogue's registers: 8 spill, 2048 rows 156 / 171 us)
+        constexpr int AHEAD = 6;
         const int used = (chunks + THREADS - 1) / THREADS;
         if (HELD == SLOTS || used <= HELD) return;
         u32x4 next[AHEAD];
@@ -436,43 +436,37 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
 
     // ---- totals of the chunks: entries, weight ----
     if (regular) {
-        // group g = i * NWV + wave of 64 keys: neighbouring groups, which are full together, are spread over the waves.  A
-        // group's keys have one sign; group SPAN / 64 starts with zero, the last group has one key.  (Few instructions a
-        // group: every wave looks through 16 of them, or 22.)
-        unsigned n[PER_WAVE];
+        // A lane lists the occupied ones among RUN neighbouring bins; where its part begins is a scan of the lanes' counts.  The
+        // first half of the lanes take the positive plane from its top (zero the last), the others the negative one.
+        const bool minus = wave >= NWV / 2;                  // (uniform)
+        const int g = minus ? tid - THREADS / 2 : SPAN / RUN - tid;
+        unsigned n[RUN], held = 0;
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) {
-            const int g = i * NWV + wave;                    // (uniform)
-            const unsigned* at = bins + (g < SPAN / 64 ? SPAN - g * 64 : NEGATIVE + min(g * 64 - SPAN, SPAN - 63));
-            n[i] = at[g < SPAN / 64 ? -lane : lane];
-            if ((i + 1) * NWV > REGULAR_KEYS / 64) n[i] = g > REGULAR_KEYS / 64 ? 0u : g == REGULAR_KEYS / 64 ? (lane == 63 ? n[i] : 0u) : n[i];
-        }
-        if (wave == SPAN / 64 % NWV && lane == 0) n[SPAN / 64 / NWV] = bins[0];
-        unsigned held = 0;
+        for (int e = 0; e < RUN; e += 4) {
+            const u32x4 x = *(const u32x4*)(bins + (minus ? NEGATIVE : 0) + min(max(g * RUN + e, 0), SPAN));
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) {
-            const unsigned c = (unsigned)__popcll(__builtin_amdgcn_ballot_w64(n[i] != 0u));
-            if (lane == i) held = c;
+            for (int i = 0; i < 4; ++i) {
+                const int bin = g * RUN + e + i;
+                n[e + i] = bin <= SPAN && bin >= (minus ? 1 : 0) ? x[i] : 0u;
+            }
         }
-        if (lane < PER_WAVE) sh.cnt[lane * NWV + wave] = held;
+#pragma unroll
+        for (int e = 0; e < RUN; ++e) held += n[e] != 0u;
+        const unsigned incl = wave_scan(held);
+        if (lane == 63) sh.wave_tot[wave] = incl;
         __syncthreads();
-        // where each group's keys go in the list: a scan over the groups, in every wave
-        u32x4 g = *(const u32x4*)&sh.cnt[lane * 4];
-        if (lane * 4 >= PER_WAVE * NWV) g = (u32x4){0u, 0u, 0u, 0u};
-        const unsigned upto = wave_scan(g[0] + g[1] + g[2] + g[3]);
-        n_pos = (int)from_lane(upto, 63);
-        unsigned base = upto - (g[0] + g[1] + g[2] + g[3]);
-        const int j = wave & 3;
-        base += (j > 0 ? g[0] : 0u) + (j > 1 ? g[1] : 0u) + (j > 2 ? g[2] : 0u);
+        const unsigned upto = wave_scan(lane < NWV ? sh.wave_tot[lane & (NWV - 1)] : 0u);
+        n_pos = (int)from_lane(upto, NWV - 1);
+        unsigned short* out = sh.patterns + (from_lane(lane_before(upto), wave) + incl - held);
+        const unsigned bits0 = (minus ? 0x8000u : 0u) + MAG_LO - 1u + g * RUN;
+        if (minus) {
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) {
-            const uint64_t any = __builtin_amdgcn_ballot_w64(n[i] != 0u);
-            if (any == 0) continue;
-            const unsigned before = __builtin_amdgcn_mbcnt_hi((unsigned)(any >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)any, 0u));
-            const int g = i * NWV + wave;
-            const unsigned bits = g < SPAN / 64 ? MAG_HI - 1u - g * 64 - lane : g == REGULAR_KEYS / 64 ? 0x8000u + MAG_HI - 1u
-                                                                                                  : 0x8000u + MAG_LO - 1u + (g * 64 - SPAN) + lane;
-            if (n[i]) sh.patterns[from_lane(base, (i * NWV + wave) >> 2) + before] = (unsigned short)(bits == 0x8000u + MAG_LO - 1u ? 0u : bits);
+            for (int e = 0; e < RUN; ++e)
+                if (n[e]) *out++ = (unsigned short)(bits0 + e);
+        } else {
+#pragma unroll
+            for (int e = RUN - 1; e >= 0; --e)
+                if (n[e]) *out++ = (unsigned short)(e == 0 && g == 0 ? 0u : bits0 + e);
         }
         __syncthreads();
         if (n_pos > 0) m = value_at(0);
@@ -885,7 +879,7 @@ int g_force = 0;        // test hook
 // One workgroup a row, of the kind that pays (Shape).
 template <bool EPI>
 void launch_rows(const SampleArgs& a, int n_rows, hipStream_t st) {
-    const bool half = a.uncond == nullptr && (g_force ? g_force == 2 : n_rows > 256);
+    const bool half = a.uncond == nullptr && (g_force ? g_force == 2 : n_rows > (EPI ? 256 : 1024));
     if (half)
         hipLaunchKernelGGL((sample_rows_kernel<EPI, false, false>), dim3(n_rows), dim3(Shape<false>::THREADS), 0, st, a);
     else if (a.uncond == nullptr)
