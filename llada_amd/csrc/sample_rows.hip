@@ -58,10 +58,11 @@ struct SampleArgs {
 //   else   512 lanes keep the first half of the longest row, read the rest past, and read that again only when the drawn
 //          entry is not in the half they hold; half the LDS, so two workgroups share a CU and one's reading goes on under
 //          the other's searches.
-// Both sides, us a call (whole / half): 256 rows 33 / 39, 512 57 / 59, 1024 99 / 98, 1536 138 / 130, 2048 178 / 161: by half
-// from there on; with the epilogue 256 rows 34 / 38, 512 61 / 56, 2048 194 / 148: past one row a CU.  Guided rows are
-// always kept whole: combining is arithmetic, which a second workgroup does not hide (256 rows 57 / 76, 2048 341 / 372 when
-// both existed).
+// Both sides, us a call (whole / half), 126464 entries: 256 rows 33 / 39, 512 57 / 59, 1024 99 / 98, 1536 138 / 130, 2048
+// 178 / 161: by half from there on; with the epilogue 256 rows 34 / 38, 512 61 / 56, 2048 194 / 148: past one row a CU.
+// Guided rows of that length are always kept whole: combining is arithmetic, which a second workgroup does not hide (256
+// rows 57 / 76, 2048 341 / 372 when both existed).  Rows that fit the half are held whole by it, guided ones too: 50257
+// entries, 32 rows 18.8 / 16.4, 1500 rows 93 / 62; 1000 entries 12.1 / 11.9, 59 / 35.
 template <bool WHOLE_>
 struct Shape {
     static constexpr bool WHOLE = WHOLE_;
@@ -186,19 +187,30 @@ __device__ __forceinline__ u32x4 combine(u32x4 c, u32x4 u, float cfg1) {
 }
 
 // Entries v0 .. v0 + 7 of a row as the draw sees them, one at a time: combined under guidance; -inf for what lies outside the
-// row and for the entry that is taken out of everything (EOS removed before the draw).
+// row and for the entry that is taken out of everything (EOS removed before the draw).  (Indexes clamped into the row and
+// no branches: the eight loads travel together.)
 template <bool EPI>
 __device__ __forceinline__ u32x4 row_chunk(const bf16_t* lc, const bf16_t* lu, int v0, int vocab, float cfg1, int excluded) {
-    u32x4 t = {0u, 0u, 0u, 0u};
+    auto fetch = [&](const bf16_t* row) {
+        bf16_t x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = row[min(max(v0 + e, 0), vocab - 1)];
+        u32x4 t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = (unsigned)x[2 * e] | (unsigned)x[2 * e + 1] << 16;
+        return t;
+    };
+    u32x4 t = fetch(lc);
+    if (lu) {
+        asm volatile("" : "+v"(t)::"memory");        // (one row's entries after the other's: eight registers fewer)
+        t = combine(t, fetch(lu), cfg1);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int v = v0 + e;
-        unsigned bits = 0xFF80u;
-        if (v >= 0 && v < vocab && !(EPI && v == excluded)) {
-            bits = lc[v];
-            if (lu) bits = f32_to_bf16(cfg_combine(bf16_to_f32((bf16_t)bits), bf16_to_f32(lu[v]), cfg1));
-        }
-        t[e >> 1] |= bits << (16 * (e & 1));
+        const bool out = v < 0 || v >= vocab || (EPI && v == excluded);
+        const unsigned keep = out ? ((e & 1) ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu, put = out ? ((e & 1) ? 0xFF800000u : 0x0000FF80u) : 0u;
+        t[e >> 1] = (t[e >> 1] & keep) | put;
     }
     return t;
 }
@@ -355,8 +367,15 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     });
     __syncthreads();
     if (tid == 0) bins[0] += bins[NEGATIVE];     // zero of either sign (the test below holds before and after)
-    // clamped bins that are not empty: zeros and -inf are as good as binned, anything else makes the row irregular
-    if (bins[0] + bins[NEGATIVE] + bins[SPAN + 1] + bins[NEGATIVE + SPAN + 1] != 0u) {
+    // clamped bins that hold more than what was put there for entries that do not count: zeros and -inf are as good as
+    // binned, anything else makes the row irregular
+    unsigned padded = (unsigned)(chunks * 8 - V) + (EPI && excl_all >= 0 ? 1u : 0u);
+    if constexpr (HELD < SLOTS) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (odd[k] >= HELD * THREADS && (k == 0 || odd[k] != odd[0]) && (k < 2 || odd[k] != odd[1])) padded += 8u;
+    }
+    if (bins[0] + bins[NEGATIVE] + bins[SPAN + 1] + bins[NEGATIVE + SPAN + 1] != padded) {
         // smallest magnitude above zero, largest positive pattern, largest negative one but -inf
         const u16x2 one = {1, 1}, minus_inf = {0xFF80, 0xFF80};
         u16x2 least = {0xFFFF, 0xFFFF}, neg = {0, 0};
@@ -879,13 +898,17 @@ int g_force = 0;        // test hook
 // One workgroup a row, of the kind that pays (Shape).
 template <bool EPI>
 void launch_rows(const SampleArgs& a, int n_rows, hipStream_t st) {
-    const bool half = a.uncond == nullptr && (g_force ? g_force == 2 : n_rows > (EPI ? 256 : 1024));
-    if (half)
+    const bool guided = a.uncond != nullptr;
+    const bool fits = a.vocab <= Shape<false>::HELD * Shape<false>::THREADS * 8 - 7;      // in half a row, wherever it starts
+    const bool half = fits ? g_force != 1 : !guided && (g_force ? g_force == 2 : n_rows > (EPI ? 256 : 1024));
+    if (half && guided)
+        hipLaunchKernelGGL((sample_rows_kernel<EPI, false, true>), dim3(n_rows), dim3(Shape<false>::THREADS), 0, st, a);
+    else if (half)
         hipLaunchKernelGGL((sample_rows_kernel<EPI, false, false>), dim3(n_rows), dim3(Shape<false>::THREADS), 0, st, a);
-    else if (a.uncond == nullptr)
-        hipLaunchKernelGGL((sample_rows_kernel<EPI, true, false>), dim3(n_rows), dim3(Shape<true>::THREADS), 0, st, a);
-    else
+    else if (guided)
         hipLaunchKernelGGL((sample_rows_kernel<EPI, true, true>), dim3(n_rows), dim3(Shape<true>::THREADS), 0, st, a);
+    else
+        hipLaunchKernelGGL((sample_rows_kernel<EPI, true, false>), dim3(n_rows), dim3(Shape<true>::THREADS), 0, st, a);
 }
 
 int check_sampling(const char* who, const llada_sampling* s) {

@@ -307,3 +307,23 @@ def test_ties_and_the_last_entry_of_a_long_row(lib):
     flat = torch.full((len(places), V), 0.5).cuda().to(torch.bfloat16)
     u = (np.array(places) + 0.5) / V
     assert sample_tokens(flat, uniforms=torch.from_numpy(u).cuda()).tolist() == places
+
+
+@pytest.mark.parametrize("V", [65528, 65529, 65530, 65536, 65543])
+@pytest.mark.parametrize("shift", [0, 5])
+def test_around_the_length_that_half_a_row_holds(lib, V, shift):
+    from llada_amd import sample_tokens
+    n = 4
+    flat = torch.full((n * (V + 8) + 8,), 9.0).cuda().to(torch.bfloat16)      # what stands between the rows would win
+    x = flat.as_strided((n, V), (V + 8, 1), shift)
+    x.copy_(logits(V, n, V))
+    x[1, V - 1] = 30.0
+    u = uniforms(V, n)
+    tok = check(x, u, top_p=0.97)
+    assert tok[1] == V - 1
+    un = flat.clone().as_strided((n, V), (V + 8, 1), shift)
+    un.copy_(logits(V + 1, n, V))
+    both = sample_tokens(x, 0.8, top_k=30, uniforms=torch.from_numpy(u).cuda(), uncond_logits=un, cfg_scale=1.5)
+    d = ((x.float() - un.float()).to(torch.bfloat16).float() * 2.5).to(torch.bfloat16)
+    first = (un.float() + d.float()).to(torch.bfloat16)
+    assert torch.equal(both, sample_tokens(first, 0.8, top_k=30, uniforms=torch.from_numpy(u).cuda()))
