@@ -12,7 +12,12 @@
 // worked on and the next tile's values during the next scores; there is no LDS staging and no barrier in the loop.
 // Codes become bf16 exactly (e4m3: one conversion for two codes; int8: three instructions for two); a tile's
 // key scale goes into the multiplier of the scores, its value scale, a power of two 2^e, into the exponent of the
-// probabilities (p 2^e = 2^(s - m + e)), so neither costs an instruction per element.
+// probabilities (p 2^e = 2^(s - m + e)), so neither costs an instruction per element.  Their sum is taken back by 2^-e: it would
+// lose the keys whose p 2^e the exponential flushes (below 2^-126), so no more than 2^-64 or 2^64 goes in before the sum: the
+// outputs have a unit, a power of two, and e counts from there.  Larger scales raise the unit (outputs stay finite up to the
+// largest bf16 values), smaller ones go into the probabilities in bf16, after the sum (what flushes there is below 2^-117 of a
+// unit); a wave that has summed nothing takes a tiny tile's scale for its unit.
+// (Fresh rows carry no scale; like the bf16 attention's, sums over them are finite for values up to 2^96.)
 //
 // Measured, 32 heads (kernel times): 32 queries on 32 x 4096 tokens 186 us (1.08 GB: 5.8 TB/s, the memory's rate), on
 // 8 x 384 8.6 us and on 1 x 384 7.8 us (latency: a few tiles a wave), 64 on 8 x 1150 int8 24 us (one workgroup a CU: the
@@ -86,14 +91,20 @@ struct Kv8Attn {
 
 // A wave's state over the tiles it has swept.
 struct Softmax {
-    f32x16 o[4];
+    f32x16 o[4];              // in units of 2^unit
     float m, l;
+    int unit;
 };
+
+// The most of a tile's value scale that goes into the exponent of its probabilities: these then stay normal numbers
+// down to 2^-62 of the largest, and finite.
+constexpr int FOLD = 64;
 
 // One tile's scores -> probabilities, the running maximum and sum brought up to date.  s: raw scores (lane: query
 // lane & 31; register 4 c + e of s[kb]: key 32 kb + 8 c + 4 (lane >> 5) + e); valid: bit per key; sc: multiplier into the
-// log2 domain; ve: exponent of the tile's value scale.
-__device__ __forceinline__ void softmax_tile(f32x16 (&s)[2], uint64_t valid, float sc, float ve, float inv_vs, Softmax& w,
+// log2 domain; ve: exponent put into the probabilities (at most FOLD either way, so that the sum misses no key that counts),
+// inv_vs: 2^-ve; over: the outputs' unit has risen by 2^over; under: what the probabilities take besides ve, after their sum.
+__device__ __forceinline__ void softmax_tile(f32x16 (&s)[2], uint64_t valid, float sc, float ve, float inv_vs, int over, int under, Softmax& w,
                                              bf16x8 (&pb)[2][2], int hg) {
     if (valid != ~0ull) {
         const uint64_t mine = valid >> (4 * hg);
@@ -112,10 +123,11 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[2], uint64_t valid, flo
     // the reference maximum moves only when it has risen by more than 2^8: the 64 multiplies of the
     // accumulators are then rare, and probabilities up to 2^8 are as exact as those below 1
     const float m_cand = fmaxf(w.m, mx);
-    if (__builtin_amdgcn_ballot_w64(m_cand > w.m + 8.0f) != 0) {
-        const float alpha = __builtin_amdgcn_exp2f(w.m - (m_cand == -INFINITY ? 0.f : m_cand));
+    if ((__builtin_amdgcn_ballot_w64(m_cand > w.m + 8.0f) | (unsigned)over) != 0) {
+        float alpha = __builtin_amdgcn_exp2f(w.m - (m_cand == -INFINITY ? 0.f : m_cand));
         w.m = m_cand;
         w.l *= alpha;
+        alpha = __builtin_ldexpf(alpha, -over);
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -132,6 +144,12 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[2], uint64_t valid, flo
             pb[kb][e >> 3][e & 7] = (__bf16)p;
         }
     w.l = __builtin_fmaf(sum, inv_vs, w.l);
+    if (under != 0) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pb[kb][e >> 3][e & 7] = (__bf16)__builtin_ldexpf((float)pb[kb][e >> 3][e & 7], under);
+    }
 }
 
 // NQ query groups of 32 and 4 / NQ key groups per workgroup: few queries -> the waves share the queries and deal the
@@ -189,6 +207,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
         for (int e = 0; e < 16; ++e) w.o[i][e] = 0.f;
     w.m = -INFINITY;
     w.l = 0.f;
+    w.unit = 0;
 
     // units of this workgroup: [u_begin, u_end) of the fresh tiles, then the cached ones; unit u_begin + i is key group i % NK's
     const int n_fresh = a.n_units - a.n_cached;
@@ -295,7 +314,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
                 hold();
             }
             bf16x8 pb[2][2];
-            softmax_tile(s, unmasked & there, a.scale_log2e, 0.f, 1.f, w, pb, hg);
+            softmax_tile(s, unmasked & there, a.scale_log2e, 0.f, 1.f, 0, 0, w, pb, hg);
             const int q4 = (lane & 15) >> 2, p4 = lane & 3, g1 = (lane >> 4) & 1;
             const unsigned char* const vrow = v_lds + (4 * hg + q4) * 256 + 32 * g1 + 8 * p4;
             s16x4 vf[2][4][2];
@@ -356,8 +375,22 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
         ks_next = scales[2 * tn];
         vs_next = scales[2 * tn + 1];
         bf16x8 pb[2][2];
-        const float ve = (float)((int)(__float_as_uint(vscale) >> 23) - 127);
-        softmax_tile(s, valid, a.scale_log2e * kscale, ve, __uint_as_float((254u << 23) - __float_as_uint(vscale)), w, pb, hg);
+        // value scale 2^(e + unit), e uniform and, values of ordinary sizes all over, never past FOLD
+        int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(vscale) >> 23)) - 127 - w.unit, over = 0, under = 0;
+        if (__builtin_expect((unsigned)(e + FOLD) > 2u * FOLD, 0)) {
+            if (__builtin_amdgcn_ballot_w64(w.m != -INFINITY) == 0) {               // nothing has been summed: any unit will do
+                w.unit += e;
+                e = 0;
+            } else if (e > 0) {
+                over = e - FOLD;
+                w.unit += over;
+                e = FOLD;
+            } else {
+                under = e + FOLD;
+                e = -FOLD;
+            }
+        }
+        softmax_tile(s, valid, a.scale_log2e * kscale, (float)e, __uint_as_float((unsigned)(127 - e) << 23), over, under, w, pb, hg);
         if (valid != ~0ull) {          // zero codes under masked keys: 0 * NaN would reach the sums
             const uint64_t mine = valid >> (4 * hg);
 #pragma unroll
@@ -385,7 +418,18 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
     unsigned char* const slice = lds + wave * SLICE;
 
     // ---- the key groups' results meet in LDS and are summed at their common maximum ----
-    const float l_tot = w.l + __shfl_xor(w.l, 32);
+    float l_tot = w.l + __shfl_xor(w.l, 32);
+    if (w.unit != 0) {
+        // The unit is taken back, and what keeps the outputs and their sum over all groups finite goes into the reference
+        // maximum: |o| 2^unit <= l 2^128, so with l brought to 2^-8 at most, 64 groups' outputs add up below 2^126.
+        const int g = l_tot > 0.f ? __builtin_amdgcn_frexp_expf(l_tot) + 8 : 0;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w.o[db][i] = __builtin_ldexpf(w.o[db][i], w.unit - g);
+        l_tot = __builtin_ldexpf(l_tot, -g);
+        w.m += (float)g;
+    }
     if (f_end > u_begin) __syncthreads();                               // the fresh tiles have been read
     if (hg == 0) {
         ml[(wave * QW + r) * 2] = w.m;

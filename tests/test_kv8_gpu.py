@@ -421,3 +421,37 @@ def test_output_in_the_queries_memory_but_not_in_the_blocks(lib, n, L, n_q):
     inside = block.view(-1)[: n * n_q * H * 128].view(n, n_q, H * 128)
     with pytest.raises(ValueError, match="overlaps"):
         cache.attend(0, block, block=block, out=inside)
+
+
+def scaled_blocks(seed, n, L, H, exponents):
+    """Rows whose 64-token blocks of values are N(0, 1) * 2^exponents[block % len], within bf16's finite range."""
+    x = rows(seed, n, L, H).double().view(n, L, 3, H, 128)
+    x[:, :, 1] *= 0.5
+    e = torch.tensor([exponents[(t // 64) % len(exponents)] for t in range(L)], dtype=torch.float64, device="cuda")
+    x[:, :, 2] = (x[:, :, 2] * 2.0 ** e[None, :, None, None]).clamp(-2.0 ** 127, 2.0 ** 127)
+    return x.view(n, L, -1).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("nq,splits,n_q", [(0, 0, 5), (1, 3, 20), (2, 1, 70), (4, 1, 140)])
+@pytest.mark.parametrize("exponents", [(0, -100), (0, -108), (-110, 0), (-120, 0, 0), (0, -126, -118), (-100,), (-110, -104), (60, -60, 0), (80, 0),
+                                       (0, 126), (126, 0), (126,), (126, -120, 0), (70, 126, 10)])
+def test_value_blocks_of_every_size(lib, exponents, nq, splits, n_q, dtype):
+    """The weights of a block's keys do not depend on the size of its values.  Beside check_attend's bound: what the exponential
+    and the matrix unit may flush, for each of the L keys 2^-117 of the largest value."""
+    n, L, H = 2, 330, 2
+    x, y = scaled_blocks(L + n_q, n, L, H, exponents), rows(77 + n_q, n, n_q, H)
+    c = make(n, L, H, dtype)
+    c.fill(0, x)
+    try:
+        lib.llada_attn_kv8_force(nq, splits)
+        got = c.attend(0, y).double().cpu().numpy().reshape(n, n_q, H, 128)
+    finally:
+        lib.llada_attn_kv8_force(0, 0)
+    _, k, v = split(x, H)
+    k, v, q = okv.held(k, dtype), okv.held(v, dtype), split(y, H)[0]
+    want, spread = okv.attend(q, k, v)
+    e = 130 * 2.0 ** -24 * np.sqrt((q ** 2).sum(-1)).max() * np.sqrt((k ** 2).sum(-1)).max() / np.sqrt(128) + 2.0 ** -19
+    tol = 2.0 ** -8 * (spread + np.abs(want)) + (2 * e + 2.0 ** -20) * spread + L * 2.0 ** -117 * np.abs(v).max()
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / tol)
