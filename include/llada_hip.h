@@ -237,9 +237,10 @@ int llada_forward_block(const llada_config* cfg, const llada_weights* w, const i
  * values of n_seq sequences of seq_len tokens: codes of 8 bits in blocks of 64 consecutive tokens and one head, each
  * block of keys and of values with one scale 2^k, k the smallest integer (>= -126) for which the block's largest
  * magnitude is at most 448 * 2^k (LLADA_KV_E4M3: OCP float8 e4m3) or 127 * 2^k (LLADA_KV_INT8); k = 0 for an
- * all-zero block.  code = x * 2^-k rounded to nearest even; the stored value code * 2^k is exact in bf16 (blocks whose
- * values are below 2^-117 excepted).  Infinities saturate and do not enter the scale; a NaN stays one in e4m3 and
- * becomes 0 in int8.  The order of the bytes inside is the library's own; llada_kv8_read gives the values.
+ * all-zero block.  code = x * 2^-k rounded to nearest even, and a code that would stand for 2^128 becomes the next lower one;
+ * the stored value code * 2^k is exact in bf16 (blocks whose values are below 2^-117 excepted).  Infinities saturate at the
+ * largest code and do not enter the scale; a NaN stays one in e4m3 and becomes 0 in int8.
+ * The order of the bytes inside is the library's own; llada_kv8_read gives the values.
  * ------------------------------------------------------------------------------------------- */
 #define LLADA_KV_E4M3 0
 #define LLADA_KV_INT8 1

@@ -7,7 +7,9 @@
 // (its steps are relative) and int8 at most one of its eight bits.
 //
 // Masked tokens are stored as zeros and do not enter the scale, so padding cannot coarsen its block; infinities
-// saturate and do not enter the scale either; a NaN stays a NaN in e4m3 and becomes 0 in int8, which has none.
+// saturate and do not enter the scale either; a NaN stays a NaN in e4m3 and becomes 0 in int8, which has none.  In a block of
+// nearly the largest bf16 values the largest codes would stand for 2^128: they become the next lower ones, so that every held
+// value of a finite or infinite input is finite.
 #include "kv8.h"
 
 namespace {
@@ -26,17 +28,27 @@ __device__ __forceinline__ int scale_exponent(float amax) {
     return k < -126 ? -126 : k;          // keeps the scale and its inverse normal numbers
 }
 
+// the largest exponent whose every code stands for a finite bf16 value (448 * 2^119, 127 * 2^121); at the one above it, codes
+// end at 240 and 63
+template <int TYPE>
+constexpr int TOP_EXPONENT = TYPE == LLADA_KV_E4M3 ? 119 : 121;
+template <int TYPE>
+__device__ __forceinline__ float code_limit(int k) {
+    return TYPE == LLADA_KV_E4M3 ? (k > TOP_EXPONENT<TYPE> ? 240.f : 448.f) : (k > TOP_EXPONENT<TYPE> ? 63.f : 127.f);
+}
+
 __device__ __forceinline__ float power_of_two(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }
 
-// Four values -> four codes.  RAW: all four are finite (then |x inv| is within the code's range by the choice of the scale).
+// Four values -> four codes of magnitude up to `limit`.  RAW: the block holds finite values alone and its scale is not the
+// topmost (then |x inv| is within the code's range by the choice of the scale).
 template <int TYPE, bool RAW>
-__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv) {
+__device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, float inv, float limit) {
     float x[4] = {a, b, c, d};
     if constexpr (TYPE == LLADA_KV_E4M3) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[i] *= inv;
-            if (!RAW) x[i] = x[i] != x[i] ? x[i] : __builtin_amdgcn_fmed3f(x[i], -448.f, 448.f);
+            if (!RAW) x[i] = x[i] != x[i] ? x[i] : __builtin_amdgcn_fmed3f(x[i], -limit, limit);
         }
         int r = 0;
         r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], r, false);
@@ -48,7 +60,7 @@ __device__ __forceinline__ unsigned encode4(float a, float b, float c, float d, 
         unsigned u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (!RAW) x[i] = x[i] != x[i] ? 0.f : __builtin_amdgcn_fmed3f(x[i] * inv, -127.f, 127.f);
+            if (!RAW) x[i] = x[i] != x[i] ? 0.f : __builtin_amdgcn_fmed3f(x[i] * inv, -limit, limit);
             u[i] = __float_as_uint(RAW ? __builtin_fmaf(x[i], inv, 12582912.f) : x[i] + 12582912.f);
         }
         const unsigned lo = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0400u);
@@ -78,25 +90,26 @@ __device__ __forceinline__ u16x2 halves(unsigned w) { return __builtin_bit_cast(
 
 // x: four keys x 8 dims of the keys and of the values; their codes into the tile's LDS image.
 template <int TYPE, bool RAW>
-__device__ __forceinline__ void encode_tile(const u32x4 (&x)[2][4], float ik, float iv, unsigned char* codes, int kg, int dg) {
+__device__ __forceinline__ void encode_tile(const u32x4 (&x)[2][4], const int (&k)[2], unsigned char* codes, int kg, int dg) {
+    const float ik = power_of_two(-k[0]), iv = power_of_two(-k[1]), lk = code_limit<TYPE>(k[0]), lv = code_limit<TYPE>(k[1]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         u32x2 w;
-        w[0] = encode4<TYPE, RAW>(entry(x[0][i], 0), entry(x[0][i], 1), entry(x[0][i], 2), entry(x[0][i], 3), ik);
-        w[1] = encode4<TYPE, RAW>(entry(x[0][i], 4), entry(x[0][i], 5), entry(x[0][i], 6), entry(x[0][i], 7), ik);
+        w[0] = encode4<TYPE, RAW>(entry(x[0][i], 0), entry(x[0][i], 1), entry(x[0][i], 2), entry(x[0][i], 3), ik, lk);
+        w[1] = encode4<TYPE, RAW>(entry(x[0][i], 4), entry(x[0][i], 5), entry(x[0][i], 6), entry(x[0][i], 7), ik, lk);
         *(u32x2*)(codes + kv8_key_offset(kg * 4 + i, dg * 8)) = w;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         *(unsigned*)(codes + KV8_CODES + kv8_value_offset(kg * 4, dg * 8 + e)) =
-            encode4<TYPE, RAW>(entry(x[1][0], e), entry(x[1][1], e), entry(x[1][2], e), entry(x[1][3], e), iv);
+            encode4<TYPE, RAW>(entry(x[1][0], e), entry(x[1][1], e), entry(x[1][2], e), entry(x[1][3], e), iv, lv);
 }
 
 // One workgroup = one (sequence, head, block): thread (kg, dg) holds keys 4 kg .. + 3 and dims 8 dg .. + 7 of the keys
 // and of the values, as bf16 pairs (what a cache holds is exact in bf16).  Bound by memory, 4 bytes in and 2 out per
 // channel, once the arithmetic is out of its way: the largest magnitude is taken on packed 16-bit patterns (2
-// instructions for two elements), and a block without infinities and NaNs, known from that maximum, needs no clamp: under
-// three instructions an element.  The codes cross the LDS once to leave as whole 1-KiB runs.
+// instructions for two elements), and a block without infinities, NaNs and values at the top of bf16, known from that
+// maximum, needs no clamp: under three instructions an element.  The codes cross the LDS once to leave as whole 1-KiB runs.
 // Measured, 32 heads: 16 x 4096 tokens 253 us e4m3 (1.61 GB: 6.4 TB/s; a copy on this card moves 4.9, which reads as much
 // as it writes), 8 x 1150 int8 45 us (0.23 GB; 54 with the clamp and float maxima), 1 x 384 5 us (launch and one round trip).
 template <int TYPE>
@@ -197,10 +210,10 @@ __global__ void __launch_bounds__(THREADS) kv8_write_kernel(const bf16_t* __rest
         block_largest(true, most);
     }
     const int k[2] = {scale_exponent<TYPE>(__uint_as_float(most[0] << 16)), scale_exponent<TYPE>(__uint_as_float(most[1] << 16))};
-    if (raw)
-        encode_tile<TYPE, true>(x, power_of_two(-k[0]), power_of_two(-k[1]), codes, kg, dg);
+    if (raw && k[0] <= TOP_EXPONENT<TYPE> && k[1] <= TOP_EXPONENT<TYPE>)
+        encode_tile<TYPE, true>(x, k, codes, kg, dg);
     else
-        encode_tile<TYPE, false>(x, power_of_two(-k[0]), power_of_two(-k[1]), codes, kg, dg);
+        encode_tile<TYPE, false>(x, k, codes, kg, dg);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < KV8_TILE / (16 * THREADS); ++i) {

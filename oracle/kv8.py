@@ -2,7 +2,8 @@
 
 Held values: blocks of 64 tokens and one head, scale 2^k with the smallest k >= -126 for which the block's largest finite
 magnitude is at most 448 * 2^k (e4m3) or 127 * 2^k (int8), k = 0 for a block of zeros; code = round-half-even(x * 2^-k),
-infinities saturated, NaN kept (e4m3) or 0 (int8); masked tokens are zeros."""
+a code that would stand for 2^128 replaced by the next lower one, infinities saturated, NaN kept (e4m3) or 0 (int8); masked
+tokens are zeros."""
 import numpy as np
 
 TOKENS = 64
@@ -40,7 +41,10 @@ def held(x, dtype, mask=None):
                             k += 1
                 y = part / 2.0 ** k
                 nan = np.isnan(y)
-                y = np.clip(np.where(nan, 0.0, y), -TOP[dtype], TOP[dtype])
+                top = TOP[dtype]
+                if top * 2.0 ** k >= 2.0 ** 128:          # (only where the block holds nearly the largest bf16 values)
+                    top = {"e4m3": 240.0, "int8": 63.0}[dtype]
+                y = np.clip(np.where(nan, 0.0, y), -top, top)
                 y = _round_to_grid(y, dtype) * 2.0 ** k
                 out[b, t:t + TOKENS, h] = np.where(nan, np.nan if dtype == "e4m3" else 0.0, y)
     return out

@@ -105,3 +105,13 @@ def test_a_cache_needs_a_gpu():
     from llada_amd import KVCache8
     with pytest.raises(ValueError, match="GPU memory"):
         KVCache8(1, 64, 2, device="cpu")
+
+
+@pytest.mark.parametrize("dtype,exponent,code", [("e4m3", 120, 240.0), ("int8", 122, 63.0)])
+def test_oracle_at_the_top_of_bf16(dtype, exponent, code):
+    """A code that would stand for 2^128 is the next lower one, for the largest finite value and for an infinity beside it."""
+    x = np.zeros((1, 64, 1, 128))
+    x[0, 0, 0, :3] = 255 * 2.0 ** 120, np.inf, -np.inf
+    assert np.array_equal(okv.held(x, dtype)[0, 0, 0, :3], np.array([1, 1, -1]) * code * 2.0 ** exponent)
+    x[0, 0, 0, 0] = okv.TOP[dtype] * 2.0 ** (exponent - 1)
+    assert okv.held(x, dtype)[0, 0, 0, 0] == x[0, 0, 0, 0]

@@ -455,3 +455,28 @@ def test_value_blocks_of_every_size(lib, exponents, nq, splits, n_q, dtype):
     tol = 2.0 ** -8 * (spread + np.abs(want)) + (2 * e + 2.0 ** -20) * spread + L * 2.0 ** -117 * np.abs(v).max()
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / tol)
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+def test_fill_at_the_top_of_bf16(lib, dtype):
+    """Codes that would stand for 2^128 become the next lower one: every held value is finite, infinities included."""
+    L, H = 64 * 5, 2
+    x = rows(6, 1, L, H).float().reshape(1, L, 3, H, 128)
+    top = torch.finfo(torch.bfloat16).max
+    x[0, :256] *= 2.0 ** 124
+    x[0, 3, 1, 0, 5], x[0, 4, 2, 1, 9] = top, -top
+    x[0, 64:128, 1:] = top
+    x[0, 130, 1:, :, 0], x[0, 131, 1:, :, 1], x[0, 132, 1:, :, 2] = top, float("inf"), float("-inf")
+    x[0, 133, 1:, 1, 3] = float("nan")
+    x[0, 200, 1:, :, 0] = 1.75 * 2.0 ** 127           # e4m3: the largest magnitude that fits 448 * 2^119
+    x[0, 260, 1:, 0, 0], x[0, 261, 1:, 0, 1] = 127 * 2.0 ** 121, float("inf")     # likewise int8, 127 * 2^121
+    xb = x.reshape(1, L, -1).to(torch.bfloat16)
+    c = make(1, L, H, dtype)
+    c.fill(0, xb)
+    _, k, v = split(xb, H)
+    for got, w in zip(values(c), (k, v)):
+        want = okv.held(w, dtype)
+        assert same(got, want) and not np.isinf(got).any()
+    c.update(0, xb[:, 3:4], 70)                       # requantised beside what the block holds
+    for got, w in zip(values(c), (k, v)):
+        assert same(got, okv.updated(okv.held(w, dtype), w[:, 3:4], 70, dtype)) and not np.isinf(got).any()
