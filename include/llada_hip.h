@@ -263,8 +263,9 @@ int llada_kv8_read(const void* cache, int32_t kv_type, void* k_out, void* v_out,
  * bf16 [Q | K | V] rows [n_seq * block_len], row stride block_stride, whose keys and values stand in for the cached ones of
  * the tokens block_start .. block_start + block_len - 1 (the cache is only read).  key_mask as above; what stands under a
  * masked token, NaN included, does not reach the result, and a sequence without an unmasked token gives zeros.
- * workspace (may be NULL; llada_attn_kv8_workspace_bytes; 16-byte aligned): scratch of this call with which the keys are
- * dealt over several workgroups where the queries alone would leave most CUs idle. */
+ * out may be q itself (same address, q_stride = n_heads * 128) and otherwise overlaps no input: workgroups read and write in
+ * no order.  workspace (may be NULL; llada_attn_kv8_workspace_bytes; 16-byte aligned): scratch of this call with which the keys
+ * are dealt over several workgroups where the queries alone would leave most CUs idle. */
 int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, const void* cache, int32_t kv_type, const uint8_t* key_mask,
                    void* out, int32_t n_seq, int32_t seq_len, int32_t n_heads, const void* block_qkv, int64_t block_stride,
                    int32_t block_start, int32_t block_len, void* workspace, size_t workspace_bytes, void* stream);

@@ -18,6 +18,13 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
+def _output_races(out, q, q_stride):
+    """Whether writing ``out`` (contiguous rows) could change queries that another workgroup has yet to read: it overlaps q's rows
+    without standing exactly in their places (each query's result replaces it after it has been read)."""
+    in_place = out.data_ptr() == q.data_ptr() and (q_stride == out.shape[-1] or out.shape[0] * out.shape[1] == 1)
+    return _overlap(out, q) and not in_place
+
+
 class KVCache8:
     """Keys and values of ``n_layers`` layers, ``n_seq`` sequences of ``seq_len`` tokens and ``n_heads`` heads of 128.
 
@@ -120,7 +127,7 @@ class KVCache8:
         unmasked token, no causal mask -> [n_seq, n_q, d] bf16.  ``block`` [n_seq, len, >= 3 d]: fresh [Q | K | V] rows
         whose keys and values stand in for the cached tokens from ``block_start`` on (the cache is only read); in a
         cached denoise step q and block are the same rows.  A sequence without an unmasked token gives zeros.  ``out`` may be
-        q's own memory, not the block's."""
+        q itself where q's rows are d wide and contiguous; any other overlap with what the call reads is refused."""
         at = self._layer(layer)
         if q.dim() != 3 or q.shape[1] < 1:
             raise ValueError(f"q: [{self.n_seq}, n_q, >= {self.d}] is wanted, not {list(q.shape)}")
@@ -142,6 +149,10 @@ class KVCache8:
                 raise ValueError(f"out: a contiguous bfloat16 [{self.n_seq}, {n_q}, {self.d}] on {self.device} is wanted")
             elif bx is not None and _overlap(out, bx):
                 raise ValueError("out overlaps the block's rows, which every head's queries read")
+            elif _overlap(out, self.data) or m is not None and _overlap(out, m):
+                raise ValueError("out overlaps the cache or the mask, which are read meanwhile")
+            elif _output_races(out, qx, q_stride):
+                raise ValueError("out overlaps q's rows without being q itself: queries would be overwritten before they are read")
             need = self._ws_bytes.get(n_q)
             if need is None:
                 need = self._ws_bytes[n_q] = self.lib.llada_attn_kv8_workspace_bytes(self.n_seq, n_q, self.seq_len, self.n_heads)

@@ -115,3 +115,16 @@ def test_oracle_at_the_top_of_bf16(dtype, exponent, code):
     assert np.array_equal(okv.held(x, dtype)[0, 0, 0, :3], np.array([1, 1, -1]) * code * 2.0 ** exponent)
     x[0, 0, 0, 0] = okv.TOP[dtype] * 2.0 ** (exponent - 1)
     assert okv.held(x, dtype)[0, 0, 0, 0] == x[0, 0, 0, 0]
+
+
+def test_which_outputs_race_with_the_queries():
+    torch = pytest.importorskip("torch")
+    from llada_amd.kv_cache import _output_races
+    d, rows = 256, 12
+    flat = torch.zeros(60 * d, dtype=torch.bfloat16)
+    q, wide = flat[d:d + rows * d].view(2, 6, d), flat[:rows * 3 * d].view(2, 6, 3 * d)
+    at = lambda i: flat[i:i + rows * d].view(2, 6, d)
+    assert not _output_races(q, q, d) and not _output_races(at((rows + 1) * d), q, d) and not _output_races(torch.zeros_like(q), q, d)
+    assert _output_races(at(0), q, d) and _output_races(at(d + 8), q, d) and _output_races(at(rows * d), q, d)
+    assert _output_races(at(0), wide, 3 * d) and _output_races(at(3 * d), wide, 3 * d) and not _output_races(at((3 * rows - 2) * d + 0), wide[..., :d], 3 * d)
+    assert not _output_races(wide[:1, :1, :d], wide[:1, :1], 3 * d) and _output_races(wide[:1, :2, :d], wide[:1, :2], 3 * d)

@@ -480,3 +480,28 @@ def test_fill_at_the_top_of_bf16(lib, dtype):
     c.update(0, xb[:, 3:4], 70)                       # requantised beside what the block holds
     for got, w in zip(values(c), (k, v)):
         assert same(got, okv.updated(okv.held(w, dtype), w[:, 3:4], 70, dtype)) and not np.isinf(got).any()
+
+
+def test_output_that_only_partly_covers_the_queries_is_refused(lib):
+    """Without a block too: an output in the storage of [Q | K | V] rows, one shifted against q, one over its last rows."""
+    n, L, H, n_q = 2, 100, 2, 6
+    d = H * 128
+    c = make(n, L, H, "e4m3")
+    c.fill(0, rows(90, n, L, H))
+    y = rows(91, n, n_q, H)
+    want = c.attend(0, y)
+    flat = torch.zeros((n * n_q + 4) * d, dtype=torch.bfloat16, device="cuda")
+    q = flat[d:d + n * n_q * d].view(n, n_q, d)
+    q.copy_(y[..., :d])
+    for bad_q, bad in ((y, y.view(-1)[:n * n_q * d]), (q, flat[:n * n_q * d]), (q, flat[2 * d:2 * d + n * n_q * d]), (q, flat[d + 8:d + 8 + n * n_q * d])):
+        with pytest.raises(ValueError, match="overlaps q"):
+            c.attend(0, bad_q, out=bad.view(n, n_q, d))
+    with pytest.raises(ValueError, match="overlaps the cache"):
+        c.attend(0, q, out=c.data.view(-1)[4096:4096 + 2 * n * n_q * d].view(torch.bfloat16).view(n, n_q, d))
+    after = flat[(n * n_q + 1) * d:(n * n_q + 1) * d + d]
+    assert torch.equal(c.attend(0, q, out=q), want) and not after.any()
+    one = make(1, L, H, "e4m3")                             # a single row may stand in its own [Q | K | V] row
+    one.fill(0, rows(92, 1, L, H))
+    z = rows(93, 1, 1, H)
+    want = one.attend(0, z)
+    assert torch.equal(one.attend(0, z, out=z[..., :d]), want)
