@@ -20,7 +20,9 @@ TOP_K_MAX = 2 ** 31 - 1
 
 def _top_k(k):
     """A top_k for the library's 32 bits: any larger one keeps the whole row as well (a negative one is refused there)."""
-    return k.clamp(-1, TOP_K_MAX) if isinstance(k, torch.Tensor) else max(-1, min(int(k), TOP_K_MAX))
+    if isinstance(k, torch.Tensor):        # (in a type that holds the limits: an int16 tensor's own does not)
+        return k.to(torch.float64 if k.is_floating_point() else torch.int64).clamp(-1, TOP_K_MAX)
+    return max(-1, min(int(k), TOP_K_MAX))
 
 
 def scalar_sampling(temperature, top_k, top_p, min_p, uniforms=None):

@@ -77,3 +77,16 @@ def test_scalars_out_of_range_are_refused_even_when_unused(bad):
     assert not truncates(0.7, **ok) and truncates(0.7, 5, 1.0, 0.0) and not truncates(0, 5, 0.5, 0.1)
     with pytest.raises(AssertionError):
         truncates(0, **{**ok, **bad})
+
+
+@pytest.mark.parametrize("dtype", ["int8", "uint8", "int16", "int32", "int64", "bool", "float16", "bfloat16", "float32", "float64"])
+def test_top_k_arrays_of_every_type(dtype):
+    """Wide enough for the library's limit whatever the tensor's own type holds."""
+    torch = pytest.importorskip("torch")
+    from llada_amd.sampling import _top_k
+    given = [0, 1, 1, 0] if dtype == "bool" else [0, 1, 100, 127] if dtype == "uint8" else [0, 1, 100, -3]
+    got = _top_k(torch.tensor(given, dtype=getattr(torch, dtype))).to(torch.int32)
+    assert got.tolist() == [max(g, -1) for g in given]
+    if dtype in ("int64", "float32", "float64"):
+        big = _top_k(torch.tensor([2 ** 40, -2 ** 40], dtype=getattr(torch, dtype))).to(torch.int32)
+        assert big.tolist() == [2 ** 31 - 1, -1]

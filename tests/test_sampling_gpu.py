@@ -327,3 +327,11 @@ def test_around_the_length_that_half_a_row_holds(lib, V, shift):
     d = ((x.float() - un.float()).to(torch.bfloat16).float() * 2.5).to(torch.bfloat16)
     first = (un.float() + d.float()).to(torch.bfloat16)
     assert torch.equal(both, sample_tokens(first, 0.8, top_k=30, uniforms=torch.from_numpy(u).cuda()))
+
+
+@pytest.mark.parametrize("dtype", ["int8", "uint8", "int16", "int32", "float16"])
+def test_top_k_arrays_of_narrow_types(lib, dtype):
+    from llada_amd import sample_tokens
+    x, u = logits(93, 4, 900), torch.from_numpy(uniforms(93, 4)).cuda()
+    k = torch.tensor([0, 1, 100, 127], device="cuda")
+    assert torch.equal(sample_tokens(x, top_k=k.to(getattr(torch, dtype)), uniforms=u), sample_tokens(x, top_k=k, uniforms=u))
