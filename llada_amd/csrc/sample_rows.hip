@@ -788,6 +788,37 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         // ---- generate.py:103-123 on the row's temperature-1 softmax, from the histogram ----
         const llada_remask_args& r = a.r;
         const int token = sh.token;
+        // f(entries) for every position that has some, dealt to the threads
+        auto each_position = [&](auto&& f) {
+            for (int win = 0; win < (regular ? 1 : WINDOWS); ++win) {
+                if (!regular) count_window(win);
+                const int p_lo = regular ? 0 : win * WINDOW, p_hi = regular ? n_pos : p_lo + WINDOW;
+#pragma unroll 1
+                for (int p = p_lo + tid; p < p_hi; p += THREADS) {
+                    const Entries x = entries_at(p);
+                    if (x.n) f(x);
+                }
+            }
+        };
+        // the largest value that this softmax sees: the row's, unless that is the entry it does not see, which may stand too far
+        // above the others for their exponentials to be taken from there
+        float mc = m;
+        if (m == lx_excl) {
+            mc = -INFINITY;
+            each_position([&](const Entries& x) {
+                if (seen(x.n, x.v) != 0u) mc = fmaxf(mc, x.v);
+            });
+            mc = wave_reduce_max(mc);
+            if (lane == 0) sh.conf[wave] = mc;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NWV; ++w) mc = fmaxf(mc, (float)sh.conf[w]);
+            __syncthreads();
+            s_sum = 0.0;
+            each_position([&](const Entries& x) {
+                if (seen(x.n, x.v) != 0u) s_sum += seen(x.n, x.v) * exp((double)x.v - (double)mc);
+            });
+        }
         s_sum = wave_total(s_sum);
         if (lane == 0) sh.conf[wave] = s_sum;
         __syncthreads();
@@ -795,7 +826,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
 #pragma unroll
         for (int w = 0; w < NWV; ++w) S += sh.conf[w];
         if (r.remasking == LLADA_REMASK_LOW_CONFIDENCE || r.remasking == LLADA_REMASK_HIGH_CONFIDENCE) {
-            const double dl = value == m ? 0.0 : (double)value - (double)m;
+            const double dl = value == mc ? 0.0 : (double)value - (double)mc;
             const float pf = token == excl_conf ? 0.f : (float)(exp(dl) / S);
             const bool f32 = (r.flags & LLADA_FLAG_CONF_FLOAT32) != 0;
             const float p = f32 ? pf : round_bf16(pf);
@@ -808,15 +839,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
                 const float p = round_bf16((float)(exp(dl) / S)), lp = round_bf16((float)(dl - lse));
                 return (double)round_bf16(lp * p);
             };
-            for (int win = 0; win < (regular ? 1 : WINDOWS); ++win) {
-                if (!regular) count_window(win);
-                const int p_lo = regular ? 0 : win * WINDOW, p_hi = regular ? n_pos : p_lo + WINDOW;
-#pragma unroll 1
-                for (int p = p_lo + tid; p < p_hi; p += THREADS) {
-                    const Entries x = entries_at(p);
-                    if (x.n) es += seen(x.n, x.v) * term(x.dl);
-                }
-            }
+            each_position([&](const Entries& x) {
+                if (seen(x.n, x.v) != 0u) es += seen(x.n, x.v) * term(m == mc ? x.dl : (double)x.v - (double)mc);
+            });
             es = wave_total(es);
             __syncthreads();
             if (lane == 0) sh.conf[wave] = es;

@@ -86,6 +86,21 @@ def check_rows(lg, x, be, mask_id, rule, flags, eos, eot, u, got, rows=None, pos
     assert (x0[~seen] == xs[~seen]).all() and (conf[~seen] == -np.inf).all()
 
 
+@pytest.mark.parametrize("rule", RULES[:4])
+@pytest.mark.parametrize("lead", [100.0, 900.0, 5000.0])
+def test_an_unseen_entry_far_above_the_rest(kind, rule, lead):
+    """EOT can be drawn although the confidence's softmax does not see it; that softmax has a maximum of its own."""
+    V, L, eos, eot = 3000, 6, 17, 29
+    lg = logits(8, L, V)
+    lg[:, eot] = lead
+    lg[3:, 40] = lead                                       # an equal entry that is seen
+    x = torch.full((1, L), 2999, dtype=torch.long, device="cuda")
+    u = torch.tensor([[0.1, 0.5, 0.999, 0.1, 0.6, 0.999]], dtype=torch.float64, device="cuda")
+    for T in (1e4, 1.0):
+        got = epilogue(kind, lg, x, L, 2999, rule, 2, eos, eot, u=u, T=T)
+        check_rows(lg, x, L, 2999, rule, 2, eos, eot, u, got, params=lambda b: dict(temperature=T))
+
+
 def full_rows(seed, n):
     """Rows of the framework's vocabulary, some with what the second half's bookkeeping has to get right."""
     lg = logits(seed, n, VOCAB)
