@@ -143,6 +143,9 @@ __device__ __forceinline__ double from_lane(double v, int at) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     return __builtin_bit_cast(double, (uint64_t)from_lane((unsigned)(b >> 32), at) << 32 | from_lane((unsigned)b, at));
 }
+__device__ __forceinline__ float uniform(float v) {         // the same in every lane: into a scalar register
+    return __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v)));
+}
 __device__ __forceinline__ double wave_total(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -242,7 +245,7 @@ __device__ __forceinline__ unsigned zero_halves(unsigned x) {
 // Draws the token of one row.  EPI: also leaves the row's confidence (rules of llada_remask_scores) in `conf`.
 template <bool EPI, class L, bool GUIDED>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, typename L::Shared& sh, const bf16_t* lc, const bf16_t* lu, double T, int top_k,
-                                           double top_p, double min_p, double u, int excl_all, int excl_conf, float& conf) {
+                                           double top_p, double min_p, double u, int excl_all, const int (&excl_conf)[2], float& conf) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     constexpr int THREADS = L::THREADS, NWV = L::NWV, SLOTS = L::SLOTS, HELD = L::HELD, SPAN = L::SPAN, NEGATIVE = L::NEGATIVE, WINDOW = L::WINDOW, RUN = L::RUN;
     constexpr int WINDOWS = 65536 / WINDOW;
@@ -263,14 +266,19 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
 
     __syncthreads();
 
-    // an entry the confidence's softmax does not see although it can be drawn (generate.py:100-101)
-    float lx_excl = -INFINITY;
-    if (EPI && excl_conf >= 0) {
-        lx_excl = bf16_to_f32(lc[excl_conf]);
-        if (lu) lx_excl = cfg_combine(lx_excl, bf16_to_f32(lu[excl_conf]), a.cfg1);
+    // entries the confidence's softmax does not see although they can be drawn (generate.py:100-101)
+    float lx_excl[2] = {-INFINITY, -INFINITY};
+    if constexpr (EPI) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (excl_conf[i] >= 0) {
+                lx_excl[i] = bf16_to_f32(lc[excl_conf[i]]);
+                if (lu) lx_excl[i] = cfg_combine(lx_excl[i], bf16_to_f32(lu[excl_conf[i]]), a.cfg1);
+                lx_excl[i] = uniform(lx_excl[i]);
+            }
     }
     // entries of a key that this softmax sees
-    auto seen = [&](unsigned n, float v) { return n - (v == lx_excl ? 1u : 0u); };
+    auto seen = [&](unsigned n, float v) { return n - (v == lx_excl[0] ? 1u : 0u) - (v == lx_excl[1] ? 1u : 0u); };
 
     // Chunks that are not one load: those the row covers only in part (its first or last) and the one with the entry taken out
     // of everything.  They are fetched entry by entry, apart from the others: this code runs once a row, and what it costs
@@ -800,10 +808,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
                 }
             }
         };
-        // the largest value that this softmax sees: the row's, unless that is the entry it does not see, which may stand too far
+        // the largest value that this softmax sees: the row's, unless that is an entry it does not see, which may stand too far
         // above the others for their exponentials to be taken from there
         float mc = m;
-        if (m == lx_excl) {
+        if (m == lx_excl[0] || m == lx_excl[1]) {
             mc = -INFINITY;
             each_position([&](const Entries& x) {
                 if (seen(x.n, x.v) != 0u) mc = fmaxf(mc, x.v);
@@ -827,7 +835,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         for (int w = 0; w < NWV; ++w) S += sh.conf[w];
         if (r.remasking == LLADA_REMASK_LOW_CONFIDENCE || r.remasking == LLADA_REMASK_HIGH_CONFIDENCE) {
             const double dl = value == mc ? 0.0 : (double)value - (double)mc;
-            const float pf = token == excl_conf ? 0.f : (float)(exp(dl) / S);
+            const float pf = token == excl_conf[0] || token == excl_conf[1] ? 0.f : (float)(exp(dl) / S);
             const bool f32 = (r.flags & LLADA_FLAG_CONF_FLOAT32) != 0;
             const float p = f32 ? pf : round_bf16(pf);
             conf = r.remasking == LLADA_REMASK_LOW_CONFIDENCE ? p : (f32 ? 1.0f - p : round_bf16(1.0f - p));
@@ -886,7 +894,10 @@ __global__ void __launch_bounds__(Shape<WHOLE>::THREADS, 4) sample_rows_kernel(c
     const bf16_t* lc = a.logits + (size_t)row * (size_t)a.stride;
     const bf16_t* lu = a.uncond ? a.uncond + (size_t)row * (size_t)a.stride : nullptr;
     const int ex_all = EPI && (a.r.flags & LLADA_FLAG_LOGITS_EOS_INF) ? a.r.eos_id : -1;
-    const int ex_conf = EPI && (a.r.flags & LLADA_FLAG_CONF_EOS_EOT_INF) && a.r.eot_id != ex_all ? a.r.eot_id : -1;
+    // EOT, and at temperature 0, where the noisy copy that loses EOS is the logits themselves, EOS (generate.py:100-101)
+    const bool no_eot = EPI && (a.r.flags & LLADA_FLAG_CONF_EOS_EOT_INF) != 0;
+    const int ex_conf[2] = {no_eot && a.r.eot_id != ex_all ? a.r.eot_id : -1,
+                            no_eot && !(T > 0.0) && a.r.eos_id != ex_all && a.r.eos_id != a.r.eot_id ? a.r.eos_id : -1};
     float conf = 0.f;
     sample_row<EPI, L, GUIDED>(a, lds, sh, lc, lu, T, top_k, top_p, min_p, u, ex_all, ex_conf, conf);
     if (tid != 0) return;

@@ -86,6 +86,32 @@ def check_rows(lg, x, be, mask_id, rule, flags, eos, eot, u, got, rows=None, pos
     assert (x0[~seen] == xs[~seen]).all() and (conf[~seen] == -np.inf).all()
 
 
+@pytest.mark.parametrize("rule,flags", [(r, f) for r in RULES for f in (0, 1, 2, 3, 4, 6) if not ("entropy" in r and f & 3)])
+def test_temperature_zero_is_the_plain_epilogue(kind, rule, flags):
+    """The arg-max through the sampled form (as a scalar and as a row's own temperature) gives llada_remask_scores' candidates
+    and confidences, EOS or EOT in the lead included.  (The entropy rules: where no entry is -inf; there the plain form's
+    0 * log 0 is NaN.)  Float32 forms differ by the sums' rounding: 2^-15; bf16 ones by one step."""
+    V, L, eos, eot = 4000, 16, 17, 29
+    lg = logits(flags + 3, L, V)
+    lg[1, eos], lg[2, eot], lg[3, eos] = 60.0, 61.0, 62.0
+    lg[3, eot] = 61.5
+    lg[4, eos] = lg[4].max()
+    lg[5, 33] = 250.0
+    x = torch.full((1, L), 3999, dtype=torch.long, device="cuda")
+    rs = torch.rand((1, L), device="cuda")
+    want = epilogue(kind, lg, x, L, 3999, rule, flags, eos, eot, rs=rs, plain=True)
+    for k in (dict(T=0.0), dict(arrays=(torch.zeros(1, device="cuda"), None, None, None))):
+        got = epilogue(kind, lg, x, L, 3999, rule, flags, eos, eot, rs=rs, **k)
+        assert (got[0] == want[0]).all()
+        for a, w in zip(got[1][0].astype(np.float64), want[1][0].astype(np.float64)):
+            if rule == "random":
+                assert a == w
+            elif flags & 4 and "entropy" not in rule:
+                assert abs(a - w) <= 2.0 ** -15 * max(w, 1 - w) + 1e-30, (a, w)
+            else:       # an entropy: three roundings a term and one of the sum, each at most a step apart
+                assert abs(a - w) <= 4 * 2.0 ** -7 * abs(w) + 1e-30 if "entropy" in rule else close(a, w, rule), (a, w)
+
+
 @pytest.mark.parametrize("rule", RULES[:4])
 @pytest.mark.parametrize("lead", [100.0, 900.0, 5000.0])
 def test_an_unseen_entry_far_above_the_rest(kind, rule, lead):
