@@ -382,7 +382,9 @@ int llada_sample_rows(const void* logits, const void* uncond_logits, int64_t row
                       int64_t* tokens, float* probs, void* stream);
 
 /* llada_remask_scores with the candidate tokens drawn this way instead of by Gumbel-max (args->temperature, noise and the
- * workspace are ignored): confidence is still the remasking rule on the row's whole temperature-1 softmax.
+ * workspace are ignored): confidence is still the remasking rule on the row's whole temperature-1 softmax; where that is NaN
+ * (a NaN or infinite logit, no finite one at all) so is the confidence.  Unlike there, an entry of -inf adds nothing to an entropy
+ * (there it makes the score NaN, as generate.py:113-118 does).
  * uniforms: [B, L], by position; parameter arrays: [B].  Philox counters: (0, column, row_offset + b, step).
  * logits 16-byte aligned, vocab a multiple of 8 up to 131072. */
 int llada_remask_scores_sampled(const llada_remask_args* args, const llada_sampling* sampling, void* stream);

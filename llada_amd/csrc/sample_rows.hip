@@ -89,6 +89,7 @@ struct Shape {
         unsigned total;
         int first[NWV];
         int irregular;
+        int broken;                      // epilogue: the row has a NaN or an infinity of positive sign
         int j, tied;                     // the drawn entry: the j-th of `tied` equal ones
         float value, prob;
         unsigned slot_tot[SLOTS];
@@ -261,6 +262,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
     if (tid < SLOTS) sh.slot_tot[tid] = 0u;
     if (tid == 0) {
         sh.irregular = 0;
+        sh.broken = 0;
         sh.token = -1;
     }
 
@@ -403,6 +405,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         const bool bad = min(least[0], least[1]) < MAG_LO - 1 || (unsigned)max(pos[0], pos[1]) >= MAG_HI ||
                          max(neg[0], neg[1]) >= 0x8000u + MAG_HI;
         if (__builtin_amdgcn_ballot_w64(bad) != 0 && lane == 0) sh.irregular = 1;
+        if constexpr (EPI) {
+            const bool odd_one = max(pos[0], pos[1]) >= 0x7F80 || max(neg[0], neg[1]) > 0xFF80;
+            if (__builtin_amdgcn_ballot_w64(odd_one) != 0 && lane == 0) sh.broken = 1;
+        }
     }
     __syncthreads();
     const bool regular = sh.irregular == 0;
@@ -581,7 +587,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
             sh.token = 0;
             sh.prob = 0.f;
         }
-        conf = 0.f;
+        conf = __builtin_nanf("");           // (a softmax of nothing)
         __syncthreads();
         return;
     }
@@ -833,7 +839,27 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, unsigned* bins, 
         double S = 0.0;
 #pragma unroll
         for (int w = 0; w < NWV; ++w) S += sh.conf[w];
-        if (r.remasking == LLADA_REMASK_LOW_CONFIDENCE || r.remasking == LLADA_REMASK_HIGH_CONFIDENCE) {
+        bool broken = mc == -INFINITY;               // (uniform)
+        if (sh.broken != 0) {                        // does this softmax see it?
+            bool any = false;
+            for (int c = tid; c < chunks; c += THREADS) {
+                const u32x4 t = row_chunk<EPI>(lc, lu, c * 8 - off, V, a.cfg1, excl_all);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const unsigned bits = (e & 1) ? t[e >> 1] >> 16 : t[e >> 1] & 0xFFFFu;
+                    const int v = c * 8 - off + e;
+                    any |= (bits == 0x7F80u || (bits & 0x7FFFu) > 0x7F80u) && v != excl_conf[0] && v != excl_conf[1];
+                }
+            }
+            const bool in_wave = __builtin_amdgcn_ballot_w64(any) != 0;
+            if (lane == 0) sh.first[wave] = in_wave;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NWV; ++w) broken |= sh.first[w] != 0;
+        }
+        if (broken) {
+            conf = __builtin_nanf("");               // it is NaN all over
+        } else if (r.remasking == LLADA_REMASK_LOW_CONFIDENCE || r.remasking == LLADA_REMASK_HIGH_CONFIDENCE) {
             const double dl = value == mc ? 0.0 : (double)value - (double)mc;
             const float pf = token == excl_conf[0] || token == excl_conf[1] ? 0.f : (float)(exp(dl) / S);
             const bool f32 = (r.flags & LLADA_FLAG_CONF_FLOAT32) != 0;

@@ -61,7 +61,7 @@ def close(cf, want, rule, f32=False):
     return abs(cf - want) <= 2.0 ** -23 * want if f32 else ulp_distance(np.float32(cf), np.float32(want)) <= 1
 
 
-def check_rows(lg, x, be, mask_id, rule, flags, eos, eot, u, got, rows=None, pos=None, params=None):
+def check_rows(lg, x, be, mask_id, rule, flags, eos, eot, u, got, rows=None, pos=None, params=None, broken=()):
     """Every (or the listed) logits row's candidate and confidence against the float64 restatement, the defaults elsewhere."""
     x0, conf = got
     B, L = x.shape
@@ -81,7 +81,9 @@ def check_rows(lg, x, be, mask_id, rule, flags, eos, eot, u, got, rows=None, pos
         assert x0[b, c] == t, (r, x0[b, c], t)
         if rule == "random":
             continue
-        want = osm.confidence(row, t, rule, eot if flags & 2 else -1)
+        if flags & 2 and params(b)["temperature"] == 0:     # there EOS leaves the softmax too (generate.py:100-101)
+            row[eos] = -np.inf
+        want = np.nan if r in broken else osm.confidence(row, t, rule, eot if flags & 2 else -1)
         assert close(float(conf[b, c]), want, rule, bool(flags & 4)), (r, float(conf[b, c]), want)
     assert (x0[~seen] == xs[~seen]).all() and (conf[~seen] == -np.inf).all()
 
@@ -110,6 +112,35 @@ def test_temperature_zero_is_the_plain_epilogue(kind, rule, flags):
                 assert abs(a - w) <= 2.0 ** -15 * max(w, 1 - w) + 1e-30, (a, w)
             else:       # an entropy: three roundings a term and one of the sum, each at most a step apart
                 assert abs(a - w) <= 4 * 2.0 ** -7 * abs(w) + 1e-30 if "entropy" in rule else close(a, w, rule), (a, w)
+
+
+@pytest.mark.parametrize("rule", RULES)
+@pytest.mark.parametrize("T", [0.0, 0.9])
+def test_rows_that_a_forward_broke(kind, rule, T):
+    """A softmax over a NaN, an infinity or nothing at all is NaN: so is the confidence, which the transfer then ranks
+    first, as after llada_remask_scores; the candidate is still the definition's.  A NaN in the entry that the softmax
+    does not see changes nothing."""
+    V, L, eos, eot = 2000, 9, 17, 29
+    lg = logits(5, L, V)
+    lg[1, 700] = float("nan")
+    lg[2] = -float("inf")
+    lg[3] = float("nan")
+    lg[4, [5, 1999]] = float("inf")
+    lg[5, eot] = float("nan")
+    lg[6] = -float("inf")
+    lg[6, eot] = 1.0
+    lg[7, 3:] = -float("inf")
+    lg[8, 1999] = -float("nan")
+    x = torch.full((1, L), 1999, dtype=torch.long, device="cuda")
+    u = torch.rand((1, L), dtype=torch.float64, device="cuda")
+    rs = torch.rand((1, L), device="cuda")
+    got = epilogue(kind, lg, x, L, 1999, rule, 2, eos, eot, u=u, rs=rs, T=T)
+    check_rows(lg, x, L, 1999, rule, 2, eos, eot, u, got, params=lambda b: dict(temperature=T), broken=(1, 2, 3, 4, 6, 8))
+    if rule == "random":
+        assert (got[1] == rs.cpu().numpy()).all()
+    elif T == 0.0 and "entropy" not in rule:
+        want = epilogue(kind, lg, x, L, 1999, rule, 2, eos, eot, rs=rs, plain=True)
+        assert (got[0] == want[0]).all() and (np.isnan(got[1]) == np.isnan(want[1])).all()
 
 
 @pytest.mark.parametrize("rule", RULES[:4])
