@@ -35,6 +35,7 @@ namespace {
 
 constexpr int MAX_CHUNKS = 65536 / 64;
 constexpr unsigned LLADA_STREAM_SAMPLE = 4u;
+constexpr double MAX_TEMPERATURE = 1.0e30;
 
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 typedef __attribute__((ext_vector_type(2))) short s16x2;
@@ -904,7 +905,8 @@ __global__ void __launch_bounds__(Shape<WHOLE>::THREADS, 4) sample_rows_kernel(c
         col = pos - b * a.r.L;
         if (a.r.x[pos] != a.r.mask_id || col >= a.r.block_end) return;      // the defaults stand (uniform)
     }
-    const double T = a.s.row_temperature ? (double)a.s.row_temperature[b] : a.s.temperature;
+    double T = a.s.row_temperature ? (double)a.s.row_temperature[b] : a.s.temperature;
+    if (T > MAX_TEMPERATURE) T = MAX_TEMPERATURE;
     const int top_k = a.s.row_top_k ? a.s.row_top_k[b] : a.s.top_k;
     const double top_p = a.s.row_top_p ? (double)a.s.row_top_p[b] : a.s.top_p;
     const double min_p = a.s.row_min_p ? (double)a.s.row_min_p[b] : a.s.min_p;
@@ -975,7 +977,7 @@ void launch_rows(const SampleArgs& a, int n_rows, hipStream_t st) {
 
 int check_sampling(const char* who, const llada_sampling* s) {
     LLADA_CHECK_ARG(s != nullptr, "%s: null sampling parameters", who);
-    LLADA_CHECK_ARG(s->row_temperature || (s->temperature >= 0.0 && s->temperature <= 1.0e30), "%s: temperature %g", who, s->temperature);
+    LLADA_CHECK_ARG(s->row_temperature || (s->temperature >= 0.0 && s->temperature <= MAX_TEMPERATURE), "%s: temperature %g", who, s->temperature);
     LLADA_CHECK_ARG(s->row_top_k || s->top_k >= 0, "%s: top_k %d", who, s->top_k);
     LLADA_CHECK_ARG(s->row_top_p || (s->top_p > 0.0 && s->top_p <= 1.0), "%s: top_p %g is outside (0, 1]", who, s->top_p);
     LLADA_CHECK_ARG(s->row_min_p || (s->min_p >= 0.0 && s->min_p <= 1.0), "%s: min_p %g is outside [0, 1]", who, s->min_p);

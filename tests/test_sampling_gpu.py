@@ -335,3 +335,13 @@ def test_top_k_arrays_of_narrow_types(lib, dtype):
     x, u = logits(93, 4, 900), torch.from_numpy(uniforms(93, 4)).cuda()
     k = torch.tensor([0, 1, 100, 127], device="cuda")
     assert torch.equal(sample_tokens(x, top_k=k.to(getattr(torch, dtype)), uniforms=u), sample_tokens(x, top_k=k, uniforms=u))
+
+
+def test_temperature_arrays_past_the_range(lib):
+    """An infinite temperature acts like 1e30: equal weights for all finite entries, none but the largest past min_p = 1."""
+    from llada_amd import sample_tokens
+    x, u = logits(94, 4, 900), torch.from_numpy(uniforms(94, 4)).cuda()
+    t = torch.tensor([float("inf"), 3e38, 1e30, float("inf")], device="cuda")
+    for kw in (dict(min_p=1.0), dict(min_p=0.5), dict(top_k=5), dict(top_p=0.5), dict()):
+        assert torch.equal(sample_tokens(x, t, uniforms=u, **kw), sample_tokens(x, 1e30, uniforms=u, **kw)), kw
+    assert torch.equal(sample_tokens(x, t, min_p=1.0, uniforms=u), x.float().argmax(dim=1))
