@@ -639,8 +639,8 @@ extern "C" int llada_attn_kv8(const void* q, int64_t q_stride, int32_t n_q, cons
     a.splits = (a.n_units + a.per_split - 1) / a.per_split;             // no empty run
     a.part_o = (float*)workspace;
     a.part_ml = a.splits > 1 ? a.part_o + (size_t)a.splits * a.n_rows * n_heads * KV8_HD : nullptr;
-    LLADA_CHECK_SUPPORTED(wgs * a.splits < 0x7fffffffLL && a.n_rows * n_heads * (KV8_HD / 4) / 256 < 0x7fffffffLL,
-                          "attn_kv8: grid too large");
+    LLADA_CHECK_SUPPORTED(wgs * a.splits * (NW * 64) < (1LL << 32) && (a.splits == 1 || a.n_rows * n_heads * (KV8_HD / 4) + 255 < (1LL << 32)),
+                          "attn_kv8: grid too large (a launch ends at 2^32 threads)");
     hipStream_t st = (hipStream_t)stream;
     if (kv_type == LLADA_KV_E4M3)
         launch<LLADA_KV_E4M3>(a, plan, (unsigned)(wgs * a.splits), st);

@@ -287,7 +287,7 @@ extern "C" int llada_kv8_write(const void* qkv, int64_t row_stride, const uint8_
     const int64_t n_tiles = (int64_t)n_seq * n_heads * n_blocks;
     const int first = start / KV8_TOKENS, touched = (start + len - 1) / KV8_TOKENS - first + 1;
     const int64_t grid = (int64_t)n_seq * n_heads * touched;
-    LLADA_CHECK_SUPPORTED(grid < 0x7fffffffLL, "kv8_write: grid too large");
+    LLADA_CHECK_SUPPORTED(grid * THREADS < (1LL << 32), "kv8_write: grid too large (a launch ends at 2^32 threads)");
     float* scales = (float*)cache;
     unsigned char* tiles = (unsigned char*)cache + kv8_scale_bytes(n_tiles);
     auto kernel = kv_type == LLADA_KV_E4M3 ? kv8_write_kernel<LLADA_KV_E4M3> : kv8_write_kernel<LLADA_KV_INT8>;
@@ -306,7 +306,7 @@ extern "C" int llada_kv8_read(const void* cache, int32_t kv_type, void* k_out, v
     LLADA_CHECK_SUPPORTED(kv_type == LLADA_KV_E4M3 || kv_type == LLADA_KV_INT8, "kv8_read: unknown cache type %d", kv_type);
     const int64_t n_blocks = kv8_blocks(seq_len);
     const int64_t n_tiles = (int64_t)n_seq * n_heads * n_blocks;
-    LLADA_CHECK_SUPPORTED(n_tiles < 0x7fffffffLL, "kv8_read: grid too large");
+    LLADA_CHECK_SUPPORTED(n_tiles * THREADS < (1LL << 32), "kv8_read: grid too large (a launch ends at 2^32 threads)");
     const float* scales = (const float*)cache;
     const unsigned char* tiles = (const unsigned char*)cache + kv8_scale_bytes(n_tiles);
     auto kernel = kv_type == LLADA_KV_E4M3 ? kv8_read_kernel<LLADA_KV_E4M3> : kv8_read_kernel<LLADA_KV_INT8>;

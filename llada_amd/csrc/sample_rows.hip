@@ -959,6 +959,8 @@ __global__ void __launch_bounds__(256) sample_defaults_kernel(const int64_t* __r
 
 int g_force = 0;        // test hook
 
+constexpr int32_t MAX_LAUNCH_ROWS = 1 << 21;      // of up to 1024 lanes: a launch ends at 2^32 threads
+
 // One workgroup a row, of the kind that pays (Shape).
 template <bool EPI>
 void launch_rows(const SampleArgs& a, int n_rows, hipStream_t st) {
@@ -1013,9 +1015,23 @@ extern "C" int llada_sample_rows(const void* logits, const void* uncond_logits, 
     a.row_offset = row_offset;
     a.tokens = tokens;
     a.probs = probs;
-    launch_rows<false>(a, n_rows, (hipStream_t)stream);
-    LLADA_CHECK_LAUNCH("sample_rows_kernel");
-    return LLADA_OK;
+    for (int32_t done = 0;;) {
+        const int32_t n = n_rows - done < MAX_LAUNCH_ROWS ? n_rows - done : MAX_LAUNCH_ROWS;
+        launch_rows<false>(a, n, (hipStream_t)stream);
+        LLADA_CHECK_LAUNCH("sample_rows_kernel");
+        done += n;
+        if (done == n_rows) return LLADA_OK;
+        a.logits += (int64_t)n * row_stride;
+        if (a.uncond) a.uncond += (int64_t)n * row_stride;
+        if (a.s.row_temperature) a.s.row_temperature += n;
+        if (a.s.row_top_k) a.s.row_top_k += n;
+        if (a.s.row_top_p) a.s.row_top_p += n;
+        if (a.s.row_min_p) a.s.row_min_p += n;
+        if (a.s.uniforms) a.s.uniforms += n;
+        a.row_offset += (uint32_t)n;
+        a.tokens += n;
+        if (a.probs) a.probs += n;
+    }
 }
 
 extern "C" int llada_remask_scores_sampled(const llada_remask_args* args, const llada_sampling* sampling, void* stream) {
@@ -1024,6 +1040,7 @@ extern "C" int llada_remask_scores_sampled(const llada_remask_args* args, const 
     LLADA_CHECK_ARG(r.logits && r.x && r.x0 && r.confidence, "remask_scores_sampled: null tensor");
     LLADA_CHECK_ARG(r.n_rows > 0 && r.B > 0 && r.L > 0 && r.vocab > 0, "remask_scores_sampled: bad shape");
     LLADA_CHECK_ARG(r.row_pos != nullptr || r.n_rows == (int64_t)r.B * r.L, "remask_scores_sampled: row_pos is required unless n_rows == B*L");
+    LLADA_CHECK_SUPPORTED(r.n_rows <= MAX_LAUNCH_ROWS, "remask_scores_sampled: %d rows, one launch takes %d", r.n_rows, MAX_LAUNCH_ROWS);
     LLADA_CHECK_SUPPORTED(r.vocab % 8 == 0 && r.vocab <= ROW_MAX_VOCAB, "remask_scores_sampled: vocab=%d must be a multiple of 8 up to %d", r.vocab, ROW_MAX_VOCAB);
     LLADA_CHECK_ARG((((uintptr_t)r.logits | (uintptr_t)r.uncond_logits) & 15) == 0, "remask_scores_sampled: logits must be 16-byte aligned");
     if (r.remasking < LLADA_REMASK_LOW_CONFIDENCE || r.remasking > LLADA_REMASK_RANDOM) {

@@ -36,6 +36,8 @@ class KVCache8:
             raise NotImplementedError(f"kv cache dtype {dtype!r} (one of {sorted(_lib.KV_TYPES)})")
         if min(n_seq, seq_len, n_heads, n_layers) < 1:
             raise ValueError("a cache needs at least one sequence, token, head and layer")
+        if max(n_seq, seq_len, n_heads, n_layers) >= 2 ** 31 or n_seq * n_heads * -(-seq_len // 64) >= 2 ** 31:
+            raise ValueError("sequences, tokens, heads and their 64-token blocks are counted in 32 bits")
         if torch.device(device).type != "cuda":
             raise ValueError(f"a KVCache8 lives in GPU memory, not on {device}")
         self.lib = _lib.load()

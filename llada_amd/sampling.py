@@ -50,6 +50,8 @@ def sample_tokens(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *, uni
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     rows = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     n = rows.shape[0]
+    if n > TOP_K_MAX:
+        raise ValueError(f"{n} rows: they are counted in 32 bits")
     if rows.stride(1) != 1 and vocab > 1 or (n > 1 and rows.stride(0) < vocab):
         rows = rows.contiguous()
     stride = rows.stride(0) if n > 1 else vocab

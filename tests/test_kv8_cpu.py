@@ -128,3 +128,15 @@ def test_which_outputs_race_with_the_queries():
     assert _output_races(at(0), q, d) and _output_races(at(d + 8), q, d) and _output_races(at(rows * d), q, d)
     assert _output_races(at(0), wide, 3 * d) and _output_races(at(3 * d), wide, 3 * d) and not _output_races(at((3 * rows - 2) * d + 0), wide[..., :d], 3 * d)
     assert not _output_races(wide[:1, :1, :d], wide[:1, :1], 3 * d) and _output_races(wide[:1, :2, :d], wide[:1, :2], 3 * d)
+
+
+def test_sizes_past_the_library_are_refused(lib):
+    """Sizes that 32 bits do not hold would wrap on their way into the library; launches end at 2^32 threads."""
+    from llada_amd import KVCache8, _lib
+    for sizes in ((2 ** 31, 64, 2), (1, 2 ** 32 + 64, 2), (1, 64, 2 ** 32 + 2)):
+        with pytest.raises(ValueError, match="32 bits"):
+            KVCache8(*sizes, device="cpu")
+    many = dict(n_seq=2 ** 23, H=2, stride=768)
+    assert write(lib, **many) == _lib.ERR_UNSUPPORTED
+    assert attend(lib, **many) == _lib.ERR_UNSUPPORTED
+    assert lib.llada_kv8_read(P16, 0, P16, P16, 2 ** 23, 64, 2, None) == _lib.ERR_UNSUPPORTED

@@ -90,3 +90,11 @@ def test_top_k_arrays_of_every_type(dtype):
     if dtype in ("int64", "float32", "float64"):
         big = _top_k(torch.tensor([2 ** 40, -2 ** 40], dtype=getattr(torch, dtype))).to(torch.int32)
         assert big.tolist() == [2 ** 31 - 1, -1]
+
+
+def test_epilogue_row_limit(lib):
+    """One launch ends at 2^32 threads: as many rows of 1024 lanes."""
+    from llada_amd import _lib
+    sp = _lib.Sampling(1.0, 1.0, 0.0, 0, None, None, None, None, None)
+    a = _lib.RemaskArgs(256, None, 0.0, None, 2 ** 22, 64, 256, 2 ** 11, 2 ** 11, 2, 3, 0, 0, 0, 0, 1.0, None, None, 0, 0, 0, 256, 256, None, 0)
+    assert lib.llada_remask_scores_sampled(C.byref(a), C.byref(sp), None) == _lib.ERR_UNSUPPORTED

@@ -345,3 +345,22 @@ def test_temperature_arrays_past_the_range(lib):
     for kw in (dict(min_p=1.0), dict(min_p=0.5), dict(top_k=5), dict(top_p=0.5), dict()):
         assert torch.equal(sample_tokens(x, t, uniforms=u, **kw), sample_tokens(x, 1e30, uniforms=u, **kw)), kw
     assert torch.equal(sample_tokens(x, t, min_p=1.0, uniforms=u), x.float().argmax(dim=1))
+
+
+def test_more_rows_than_one_launch_takes(lib):
+    """2^32 threads are a launch's limit; the library's uniforms, given ones and parameter arrays keep their rows."""
+    from llada_amd import sample_tokens
+    n, V = 2 ** 22 + 5, 8
+    x = torch.randn((n, V), device="cuda").to(torch.bfloat16)
+    t = torch.linspace(0.2, 2.0, n, device="cuda")
+    k = (torch.arange(n, device="cuda") % 9).to(torch.int32)
+    u = torch.rand(n, dtype=torch.float64, device="cuda")
+    p, q = torch.full((n,), 0.9, device="cuda"), torch.full((n,), 0.01, device="cuda")
+    tok, pr = sample_tokens(x, t, k, p, q, seed=3, row_offset=7, return_probs=True)
+    given = sample_tokens(x, t, k, uniforms=u)
+    for a, b in ((0, 9), (2 ** 21 - 4, 2 ** 21 + 4), (2 ** 22 - 4, n)):
+        w, v = sample_tokens(x[a:b], t[a:b], k[a:b], p[a:b], q[a:b], seed=3, row_offset=7 + a, return_probs=True)
+        assert torch.equal(tok[a:b], w) and torch.equal(pr[a:b], v)
+        assert torch.equal(given[a:b], sample_tokens(x[a:b], t[a:b], k[a:b], uniforms=u[a:b]))
+    with pytest.raises(ValueError, match="32 bits"):
+        sample_tokens(x[:1, :1].expand(2 ** 32 + 2, 1))
