@@ -569,8 +569,8 @@ void launch(const Kv8Attn& a, Plan p, unsigned grid, hipStream_t st) {
 
 extern "C" size_t llada_attn_kv8_workspace_bytes(int32_t n_seq, int32_t n_q, int32_t seq_len, int32_t n_heads) {
     if (n_seq <= 0 || n_q <= 0 || seq_len <= 0 || n_heads <= 0) return 0;
-    // + 1: a fresh block that tile borders cut sweeps one tile more
-    const Plan p = pick_plan(n_seq, n_q, n_heads, (int)kv8_blocks(seq_len) + 1, true);
+    // + 2: a fresh block that tile borders cut at both ends sweeps up to two tiles more (start 1, 65 tokens)
+    const Plan p = pick_plan(n_seq, n_q, n_heads, (int)kv8_blocks(seq_len) + 2, true);
     return p.splits > 1 ? part_bytes((int64_t)n_seq * n_q, n_heads, p.splits) : 0;
 }
 

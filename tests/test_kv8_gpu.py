@@ -505,3 +505,16 @@ def test_output_that_only_partly_covers_the_queries_is_refused(lib):
     z = rows(93, 1, 1, H)
     want = one.attend(0, z)
     assert torch.equal(one.attend(0, z, out=z[..., :d]), want)
+
+
+@pytest.mark.parametrize("L", [64 * 30, 64 * 46])
+def test_scratch_covers_a_block_cut_at_both_ends(lib, L):
+    """Two tiles more than the cache has: the scratch asked for holds the splits that the call then plans."""
+    n, H, n_q, start = 1, 2, 65, 1
+    x, y = rows(95, n, L, H), rows(96, n, n_q, H)
+    c = make(n, L, H, "e4m3")
+    c.fill(0, x)
+    a = c.attend(0, y, block=y, block_start=start)
+    c._ws_bytes[n_q] *= 2
+    assert torch.equal(c.attend(0, y, block=y, block_start=start), a)        # more scratch changes nothing: the same splits
+    check_attend(c, x, H, n_q, "e4m3", None, True, start, y)
