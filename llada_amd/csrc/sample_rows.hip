@@ -59,11 +59,12 @@ struct SampleArgs {
 //   else   512 lanes keep the first half of the longest row, read the rest past, and read that again only when the drawn
 //          entry is not in the half they hold; half the LDS, so two workgroups share a CU and one's reading goes on under
 //          the other's searches.
-// Both sides, us a call (whole / half), 126464 entries: 256 rows 33 / 39, 512 57 / 59, 1024 99 / 98, 1536 138 / 130, 2048
-// 178 / 161: by half from there on; with the epilogue 256 rows 34 / 38, 512 61 / 56, 2048 194 / 148: past one row a CU.
+// Both sides, us in a graph (whole / half), 126464 entries, temperature 0.8, min_p 0.02 (other parameters: within 3): 256 rows
+// 30.5 / 33.1, 384 46.1 / 47.2, 512 52.1 / 50.4, 768 73.8 / 70.2, 1024 92.6 / 78.8, 2048 174.6 / 139.5; with the epilogue 256
+// rows 33.8 / 37.0, 384 50.4 / 52.7, 512 56.4 / 52.6, 1024 102.3 / 88.2, 2048 193.5 / 153.3: by half from two rows a CU on.
 // Guided rows of that length are always kept whole: combining is arithmetic, which a second workgroup does not hide (256
 // rows 57 / 76, 2048 341 / 372 when both existed).  Rows that fit the half are held whole by it, guided ones too: 50257
-// entries, 32 rows 18.8 / 16.4, 1500 rows 93 / 62; 1000 entries 12.1 / 11.9, 59 / 35.
+// entries, 32 rows 18.2 / 15.6, 1500 rows 95 / 60; 1000 entries 16.6 / 11.7, 70 / 40.
 template <bool WHOLE_>
 struct Shape {
     static constexpr bool WHOLE = WHOLE_;
@@ -966,7 +967,7 @@ template <bool EPI>
 void launch_rows(const SampleArgs& a, int n_rows, hipStream_t st) {
     const bool guided = a.uncond != nullptr;
     const bool fits = a.vocab <= Shape<false>::HELD * Shape<false>::THREADS * 8 - 7;      // in half a row, wherever it starts
-    const bool half = fits ? g_force != 1 : !guided && (g_force ? g_force == 2 : n_rows > (EPI ? 256 : 1024));
+    const bool half = fits ? g_force != 1 : !guided && (g_force ? g_force == 2 : n_rows >= 512);
     if (half && guided)
         hipLaunchKernelGGL((sample_rows_kernel<EPI, false, true>), dim3(n_rows), dim3(Shape<false>::THREADS), 0, st, a);
     else if (half)

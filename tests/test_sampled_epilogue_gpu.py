@@ -196,15 +196,15 @@ def test_the_frameworks_vocabulary(kind, rule, flags):
 
 @pytest.mark.parametrize("rule,flags", [("low_confidence", 1), ("low_entropy", 3)])
 def test_more_rows_than_units_at_given_positions(lib, rule, flags):
-    """264 rows in a shuffled order of positions, with no kind forced: the form that keeps half a row and streams the rest."""
-    n, L, be = 264, 40, 33
+    """528 rows in a shuffled order of positions, with no kind forced: the form that keeps half a row and streams the rest."""
+    n, L, be = 528, 40, 33
     lg = full_rows(2, n)
-    x = torch.full((8, L), MASK, dtype=torch.long, device="cuda")
+    x = torch.full((16, L), MASK, dtype=torch.long, device="cuda")
     g = np.random.Generator(np.random.PCG64(3))
-    pos = np.concatenate([b * L + np.arange(33) for b in range(8)])
+    pos = np.concatenate([b * L + np.arange(33) for b in range(16)])
     g.shuffle(pos)
     x.view(-1)[torch.from_numpy(pos[20:30]).cuda()] = 5     # rows whose position has been decided
-    u = torch.from_numpy(g.random((8, L))).cuda()
+    u = torch.from_numpy(g.random((16, L))).cuda()
     got = epilogue(lib, lg, x, be, MASK, rule, flags, EOS, EOT, u=u, row_pos=torch.from_numpy(pos.astype(np.int32)).cuda(), top_p=0.97)
     check_rows(lg, x, be, MASK, rule, flags, EOS, EOT, u, got, rows=set(range(12)) | set(range(30, n, 13)), pos=pos,
                params=lambda b: dict(temperature=0.9, top_p=0.97))
