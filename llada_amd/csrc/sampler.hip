@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(ROW_THREADS) remask_rows_kernel(const llada_re
         bd.i = red_i[0];
 #pragma unroll
         for (int w = 1; w < NW; ++w) bd = arg_better(bd, ArgD{red_d[w], red_i[w]});
-        x0 = bd.i;
+        x0 = bd.i == 0x7fffffff ? 0 : bd.i;      // (no score compares with anything: a row of NaN)
         row.load(lc, lu, cfg1, chunks, tid, row_lds);
         if (eos_inf) row.exclude(a.eos_id, tid);
     } else {
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(256) remask_merge_kernel(const llada_remask_ar
         // temperature > 0: x0 is the Gumbel arg-max; its logit is read back (it need not be the maximum)
         ArgD bd = {gparts[(size_t)r * splits].v, gparts[(size_t)r * splits].i};
         for (int k = 1; k < splits; ++k) bd = arg_better(bd, ArgD{gparts[(size_t)r * splits + k].v, gparts[(size_t)r * splits + k].i});
-        x0 = bd.i;
+        x0 = bd.i == 0x7fffffff ? 0 : bd.i;      // (a row of NaN)
         float conf;
         if (a.remasking == LLADA_REMASK_RANDOM) {
             if (a.rand_scores) {

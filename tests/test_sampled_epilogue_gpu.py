@@ -233,3 +233,26 @@ def test_parameters_of_each_sequence(kind):
     got = epilogue(kind, lg, x, L, V - 1, "low_confidence", 0, 17, 29, u=u, arrays=(t, k, p, q))
     check_rows(lg, x, L, V - 1, "low_confidence", 0, 17, 29, u, got,
                params=lambda b: dict(temperature=float(t[b]), top_k=int(k[b]), top_p=float(p[b]), min_p=float(q[b])))
+
+
+@pytest.mark.parametrize("rule", RULES)
+def test_a_row_of_nan_under_gumbel_noise(lib, rule):
+    """llada_remask_scores with a temperature on rows where no score compares: token 0, and NaN for its confidence."""
+    from llada_amd import _lib
+    V, L = 4096, 6
+    lg = logits(41, L, V)
+    lg[1] = float("nan")
+    lg[4] = -float("nan")
+    x = torch.full((1, L), V - 1, dtype=torch.long, device="cuda")
+    rs = torch.rand((1, L), device="cuda")
+    for scratch in (True, False):
+        x0, conf = torch.full_like(x, -7), torch.full((1, L), 9.0, device="cuda")
+        ws = torch.empty(lib.llada_rows_workspace_bytes(L), dtype=torch.uint8, device="cuda")
+        a = _lib.RemaskArgs(lg.data_ptr(), None, 0.0, None, L, V, x.data_ptr(), 1, L, L, V - 1, _lib.REMASK[rule], 0, 17, 29, 0.8, None, rs.data_ptr(),
+                            3, 0, 0, x0.data_ptr(), conf.data_ptr(), ws.data_ptr() if scratch else None, ws.numel() if scratch else 0)
+        _lib.check(lib.llada_remask_scores(C.byref(a), _lib.stream_ptr()))
+        assert (x0[0, [1, 4]] == 0).all() and ((x0 >= 0) & (x0 < V)).all()
+        if rule == "random":
+            assert torch.equal(conf, rs)
+        else:
+            assert torch.isnan(conf[0, [1, 4]]).all() and torch.isfinite(conf[0, [0, 2, 3, 5]]).all()
