@@ -386,7 +386,7 @@ int llada_sample_rows(const void* logits, const void* uncond_logits, int64_t row
  * (a NaN or infinite logit, no finite one at all) so is the confidence.  Unlike there, an entry of -inf adds nothing to an entropy
  * (there it makes the score NaN, as generate.py:113-118 does).
  * uniforms: [B, L], by position; parameter arrays: [B].  Philox counters: (0, column, row_offset + b, step).
- * logits 16-byte aligned, vocab a multiple of 8 up to 131072. */
+ * logits 16-byte aligned, vocab a multiple of 8 up to 131072, up to 2^21 rows. */
 int llada_remask_scores_sampled(const llada_remask_args* args, const llada_sampling* sampling, void* stream);
 
 /* generate.py:130-134: per row b, the k = sched[b*sched_stride + step] largest confidences

@@ -22,7 +22,10 @@
 // Bound by a CU's own work on a row, 41 to 50 thousand cycles where 1024 lanes do it: the histogram 21 to 26 (its LDS
 // atomics alone 16: 64 random bins meet in the banks, 8 cycles an instruction), listing the occupied bins 4.5, their
 // weights and prefixes 5, the searches 6 (one wave, a chain of scans), the place of the token 3 to 8; from a few rows a CU
-// on by memory (Shape).  126464 entries: 32 rows 23 us, 256 guided 45 us (2.9 TB/s), 2048 rows 140 us (3.7 TB/s of rows).
+// on by memory (Shape).  126464 entries: 32 rows 24 us, 256 guided 45 us (2.9 TB/s), 2048 rows 139 us (3.7 TB/s of rows).
+// An irregular row is read again, entry by entry, for each window (4, or 8 by half), each cut and the token: 230 to 310 us for
+// up to 256 rows, 2.6 ms for 2048.  A vocabulary masked with -1e4 or the type's lowest value makes its rows irregular, one
+// masked with -inf does not.
 // Tried and dropped: reading a row twice and keeping none of it (2048 rows 198 us against the 194 of rows kept whole); a
 // wave-major order of the chunks (slower); four workgroups that count a quarter of a row each and a fifth that joins
 // their bins and goes on (32 rows 23.4 us against 23.3 in a graph, guided 44 / 39: the second launch and the fixed
