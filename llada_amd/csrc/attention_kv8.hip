@@ -96,7 +96,12 @@ struct Softmax {
     f32x16 o[4];              // in units of 2^unit
     float m, l;
     int unit;
+    bool far;                 // some query's maximum is past FAR
 };
+
+// A fused s sc - m leaves up to half a step of m in the exponent, the same for all keys: harmless until that nears the
+// exponent's range, for maxima of 2^30.  Past FAR the product is rounded before the difference, as it was for m: nothing is left.
+constexpr float FAR = 16777216.f;
 
 // The most of a tile's value scale that goes into the exponent of its probabilities: these then stay normal numbers
 // down to 2^-62 of the largest, and finite.
@@ -128,12 +133,20 @@ __device__ __forceinline__ void softmax_tile(f32x16 (&s)[2], uint64_t valid, flo
     if ((__builtin_amdgcn_ballot_w64(m_cand > w.m + 8.0f) | (unsigned)over) != 0) {
         float alpha = __builtin_amdgcn_exp2f(w.m - (m_cand == -INFINITY ? 0.f : m_cand));
         w.m = m_cand;
+        w.far = __builtin_amdgcn_ballot_w64(fabsf(m_cand) > FAR && m_cand != -INFINITY) != 0;
         w.l *= alpha;
         alpha = __builtin_ldexpf(alpha, -over);
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
             for (int e = 0; e < 16; ++e) w.o[db][e] *= alpha;
+    }
+    if (__builtin_expect(w.far, 0)) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] *= sc;
+        sc = 1.f;
     }
     const float off = ve - (w.m == -INFINITY ? 0.f : w.m);
     float sum = 0.f;
@@ -210,6 +223,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_kv8_kernel(const Kv8Attn a) {
     w.m = -INFINITY;
     w.l = 0.f;
     w.unit = 0;
+    w.far = false;
 
     // units of this workgroup: [u_begin, u_end) of the fresh tiles, then the cached ones; unit u_begin + i is key group i % NK's
     const int n_fresh = a.n_units - a.n_cached;

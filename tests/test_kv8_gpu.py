@@ -518,3 +518,56 @@ def test_scratch_covers_a_block_cut_at_both_ends(lib, L):
     c._ws_bytes[n_q] *= 2
     assert torch.equal(c.attend(0, y, block=y, block_start=start), a)        # more scratch changes nothing: the same splits
     check_attend(c, x, H, n_q, "e4m3", None, True, start, y)
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("nq,splits,n_q,fresh", [(0, 0, 5, False), (1, 3, 20, True), (2, 1, 70, False), (4, 1, 140, True)])
+@pytest.mark.parametrize("exponents", [(20,), (25,), (30,), (40,), (70, 0), (0, 45, 100), (110,)])
+def test_key_blocks_of_every_size(lib, exponents, nq, splits, n_q, fresh, dtype):
+    """Scores past what the exponential's argument resolves: the softmax is one-hot, and its one value comes back (the largest
+    probability is 1 up to a common factor: bf16 roundings of it and of the result).  Queries whose two largest scores float32
+    sums could confuse (130 * 2^-24 of |q| |k| each) are left out."""
+    n, L, H, start = 2, 330, 2, 100
+    x, y = rows(97, n, L, H).double().view(n, L, 3, H, 128), rows(98, n, n_q, H)
+    e = torch.tensor([exponents[(t // 64) % len(exponents)] for t in range(L)], dtype=torch.float64, device="cuda")
+    x[:, :, 1] *= 2.0 ** e[None, :, None, None]
+    x = x.view(n, L, -1).to(torch.bfloat16)
+    f = rows(99, n, 90, H)
+    if fresh:
+        f.view(n, 90, 3, H, 128)[:, :, 1] *= 2.0 ** max(exponents)
+    c = make(n, L, H, dtype)
+    c.fill(0, x)
+    try:
+        lib.llada_attn_kv8_force(nq, splits)
+        got = c.attend(0, y, block=f if fresh else None, block_start=start if fresh else 0).double().cpu().numpy().reshape(n, n_q, H, 128)
+    finally:
+        lib.llada_attn_kv8_force(0, 0)
+    _, k, v = split(x, H)
+    k, v, q = okv.held(k, dtype), okv.held(v, dtype), split(y, H)[0]
+    if fresh:
+        _, k[:, start:start + 90], v[:, start:start + 90] = split(f, H)
+    assert np.isfinite(got).all()
+    score = np.einsum("bqhd,bkhd->bhqk", q, k) / np.sqrt(128)
+    top = np.sort(score, axis=3)[..., -2:]
+    size = np.sqrt((q ** 2).sum(-1)).transpose(0, 2, 1)[..., None] * np.sqrt((k ** 2).sum(-1)).transpose(0, 2, 1)[:, :, None, :] / np.sqrt(128)
+    clear = top[..., 1] - top[..., 0] > 2 * 130 * 2.0 ** -24 * size.max(axis=3) + 40
+    at = score.argmax(axis=3)
+    assert clear.mean() > 0.9
+    for b in range(n):
+        for h in range(H):
+            rows_ = np.nonzero(clear[b, h])[0]
+            want = v[b, at[b, h, rows_], h]
+            assert (np.abs(got[b, rows_, h] - want) <= 2.0 ** -7 * np.abs(want) + 1e-12).all()
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+def test_tiny_keys_under_a_mask(lib, dtype):
+    """Scores that vanish (key scales down to 2^-126 take the scores' multiplier below the normal numbers): equal weights for the
+    unmasked keys, none for the others."""
+    n, L, H, n_q = 2, 200, 2, 9
+    m = left_mask(n, L, 5)
+    m[1, 100:] = 0
+    for e in (-100, -126):
+        x = rows(100, n, L, H).double().view(n, L, 3, H, 128)
+        x[:, :, 1] *= 2.0 ** e
+        check_attend(make(n, L, H, dtype), x.view(n, L, -1).to(torch.bfloat16), H, n_q, dtype, m, False, 0)
