@@ -263,6 +263,7 @@ int llada_kv8_read(const void* cache, int32_t kv_type, void* k_out, void* v_out,
  * bf16 [Q | K | V] rows [n_seq * block_len], row stride block_stride, whose keys and values stand in for the cached ones of
  * the tokens block_start .. block_start + block_len - 1 (the cache is only read).  key_mask as above; what stands under a
  * masked token, NaN included, does not reach the result, and a sequence without an unmasked token gives zeros.
+ * Sums over fresh values past 2^96 may overflow, as over llada_attn_bidir_queries_bf16's; cached ones do not.
  * out may be q itself (same address, q_stride = n_heads * 128) and otherwise overlaps no input: workgroups read and write in
  * no order.  workspace (may be NULL; llada_attn_kv8_workspace_bytes; 16-byte aligned): scratch of this call with which the keys
  * are dealt over several workgroups where the queries alone would leave most CUs idle. */

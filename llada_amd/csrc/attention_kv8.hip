@@ -21,10 +21,10 @@
 //
 // Measured, 32 heads, us a call among others (the kernel traced alone, with the profiler's gaps, takes 1 to 8 % more): 32
 // queries on 32 x 4096 tokens 186 (1.08 GB: 5.8 TB/s, the memory's rate), on 8 x 384 9.3 and on 1 x 384 9.2 (kernels 9.7
-// and 8.0, latency: a few tiles a wave), 64 on 8 x 1150 int8 23.7 (one workgroup a CU: the wave's own chain of load, convert,
-// scores, exponentials, values), 1 on 5 x 2049 int8 19.6 (likewise), 321 on 8 x 769 54 (0.60 PFLOP/s: the chain again, two
-// waves a SIMD, each loading and converting every tile for itself, 1.5 rounds of workgroups), 256 on 16 x 2176 178 in a
-// graph (0.82 PFLOP/s).  Keeping tiles of extreme value scales right costs the others up to 1 % (8 x 512, 128 queries: 4 %).
+// and 8.0, latency: a few tiles a wave), 64 on 8 x 1150 int8 24 (one workgroup a CU: the wave's own chain of load, convert,
+// scores, exponentials, values), 1 on 5 x 2049 int8 19.7 (likewise), 321 on 8 x 769 55 (0.59 PFLOP/s: the chain again, two
+// waves a SIMD, each loading and converting every tile for itself, 1.5 rounds of workgroups), 256 on 16 x 2176 181 in a
+// graph (0.81 PFLOP/s).  Keeping extreme value scales and scores right costs all others up to 2 % (8 x 512, 128 queries: 4 %).
 // Tried and dropped: workgroups of 8 waves (level or slower, but for 64 queries on 8 x 1150: 25.0 us against
 // the 27.5 of that time), a fresh tile in halves of 32 keys with one half's exponentials under the other's products
 // (level; on cached tiles its registers spill), raised wave priority around the products (level), fresh tiles last (a
